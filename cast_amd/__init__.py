@@ -29,6 +29,9 @@ _LAZY = {
     "gather_cache": "verify",
     "topk_marginals": "draft",
     "build_trees": "draft",
+    "paged_append": "paged",
+    "paged_attention": "paged",
+    "paged_workspace_bytes": "paged",
     "build_tree_device": "draft",
 }
 

@@ -24,6 +24,8 @@ FLAG_BAD_PACK = 1
 FLAG_BAD_OFFSETS = 2
 FLAG_BAD_PARENT = 4
 FLAG_TOO_LONG = 8
+FLAG_BAD_PAGE = 16
+FLAG_BAD_POSITION = 32
 
 BF16, FP32, FP64, FP16 = 0, 1, 2, 3
 
@@ -50,6 +52,11 @@ SIGNATURES = {
     "cast_tree_attn_default_split": ([_I32, _I32, _I32, _I32, _I32, _I32, _I32], _I32),
     "cast_store_append": ([_P] * 4 + [_I32] + [_P] * 2 + [_I32] + [_P] * 3 + [_I32] * 5 + [_I64] * 10 +
                           [_I32, _P, _P], ctypes.c_int),
+    "cast_paged_append": ([_P] * 4 + [_I32, _P, _I64, _I32, _I32, _I32, _P, _P, _I32, _I32, _P, _P, _I32] + [_P] * 6 +
+                          [_I64, _I32, _I32, _I32, _P, _I32, _I32, _I32] + [_I64] * 16 + [_I32, _P, _P], ctypes.c_int),
+    "cast_paged_attn_fwd": ([_P] * 6 + [_I64, _I32, _I32, _I32, _P, _I32, _I32, _I32, _I32] + [_I64] * 10 +
+                            [_I32, ctypes.c_float, ctypes.c_float, _I32, _I32, _P, _SZ, _P, _P], ctypes.c_int),
+    "cast_paged_attn_workspace_size": ([_I32] * 9, _SZ),
     "cast_draft_topk": ([_P, _I64, _I32, _I32, _I32, _I32, _P, _P, _I32, _P, _SZ, _P], ctypes.c_int),
     "cast_draft_topk_workspace_size": ([_I32, _I32, _I32, _I32, _I32], _SZ),
     "cast_build_trees_uniform": ([_P, _P, _I32, _I32, _I32, _I32, _I32] + [_P] * 7, ctypes.c_int),
@@ -145,4 +152,8 @@ def raise_device_flags(flags, what):
         parts.append("a parent index is not in [-1, own index)")
     if flags & FLAG_TOO_LONG:
         parts.append("a request's keys exceed the kernel's row addressing (2^24 rows / 2 GiB per source)")
+    if flags & FLAG_BAD_PAGE:
+        parts.append("a page id is outside the pool")
+    if flags & FLAG_BAD_POSITION:
+        parts.append("a position is outside the rotation tables")
     raise ValueError(f"{what}: " + "; ".join(parts))

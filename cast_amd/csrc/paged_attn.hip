@@ -1,0 +1,798 @@
+// K7: attention of one new token per request over a KV cache of pages.
+//
+// The ordinary decode step beside the tree verification of K2 (what the
+// reference's autoregressive loop, cast_trees/decode.py:211-231, leaves to
+// the model's attention): request b's query sees the keys of slots
+// [start, len), len = seq_len[b], start = len - window where a window is set,
+//   o = sum_t softmax_t(f(scale q . k_t)) v_t,   f(s) = cap tanh(s / cap)
+// with a cap, the identity without.  Slot t lies in page
+// table[b][t / page_size] at offset t % page_size.  Query head h reads KV head
+// h / (Hq / Hkv).
+//
+// Bound by the K and V bytes: 4 D bytes a key and KV head in 16 bits against
+// 4 D G flops.  The G query heads of a KV head are the columns of 16-wide
+// matrix products, so each key is read once for all of them and the products
+// cost a tenth of the time its bytes take.
+//
+// A work item is (request, KV head, block of 16 query heads, run of key
+// tiles); its four waves take 16 KB of keys in turn, each on its own with its
+// own running maximum and sum, and join through LDS at the end.  No operand
+// goes through LDS:
+//   S^T = K Q^T   a lane holds 16-byte chunks of one key's row, as the
+//                 product's K-side operand wants them;
+//   O^T += V^T P^T  a lane holds D/16 elements of 8 keys (16-byte chunks,
+//                 neighbouring lanes reading neighbouring chunks of a row),
+//                 which v_perm turns into 8 keys of each element; the keys it
+//                 takes are those whose weights the first product left in its
+//                 registers, and the order of the head dim over the operand's
+//                 rows is free.
+// fp32 runs both products on the fp32 matrix instruction.  16-bit weights are
+// two terms (p - round(p) is the second), so that they keep float precision
+// where the matrix pipes have room; V rows of masked keys are zeroed, as
+// memory behind the last token may hold anything.
+//
+// The next tile's loads are issued before the current one is used; page ids
+// are loaded 64 blocks ahead.  Long requests are split over keys, each split
+// writes (O, max, sum) in float and a second kernel joins them.
+#include <limits.h>
+#include <math.h>
+
+#include <mutex>
+
+#include "cast_common.hpp"
+
+namespace cast {
+
+constexpr float kPLn2 = 0.69314718055994530942f;
+constexpr float kPLog2e = 1.44269504088896340736f;
+constexpr int kPWaves = 4;
+constexpr int kMinTiles = 2;             // fewest key tiles of an automatic split
+
+struct PagedAttnArgs {
+    const void *q, *k, *v;
+    void *out;
+    float *lse;
+    const int32_t *table, *seq_len;
+    int32_t *status;
+    int64_t table_ld, q_req, q_head, o_req, o_head;                      // elements (q, out)
+    int64_t kp_page, kp_head, kp_tok, vp_page, vp_head, vp_tok;          // bytes
+    int32_t n_pages, page_size, batch, Hq, Hkv, G, rbs, D, cap, window;  // cap: slots a table row covers
+    int32_t split;      // tiles per split asked for; 0: chosen from the lengths; INT_MAX: one split
+    int32_t slots;      // workgroups resident at once
+    float scale, softcap;   // scale: natural scale (softcap) or times log2(e)
+    int32_t *head;      // workspace: [batch] first item, [batch] splits
+    float *part_ml;     // [items][16][2] running maximum (base 2) and sum; sum < 0: a page id is bad
+    float *part_o;      // [items][16][D]
+};
+
+// ---- lanes and waves
+__device__ __forceinline__ int p_wave_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+    return x;
+}
+__device__ __forceinline__ int p_wave_sum(int x) { return __builtin_amdgcn_readlane(p_wave_scan(x), 63); }
+
+// The largest / the sum over the four lanes that share l16 = lane % 16.
+__device__ __forceinline__ float quad_max(float x) {
+    x = fmaxf(x, __shfl_xor(x, 16));
+    return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float quad_sum(float x) {
+    x += __shfl_xor(x, 16);
+    return x + __shfl_xor(x, 32);
+}
+
+// ---- formats
+struct PF32 {
+    static constexpr int kBytes = 4, kBlocks = 1;     // 16-key blocks per wave tile
+    static constexpr float kPScale = 1.f;
+    using T = float;
+};
+struct PBf16 : Bf16 {
+    static constexpr int kBytes = 2, kBlocks = 2;
+    static constexpr float kPScale = 1.f;
+    using T = uint16_t;
+    static __device__ __forceinline__ floatx4 mma16(vec8 a, vec8 b, floatx4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+};
+// fp16 weights are scaled by 2^15, so that their second term stays a normal
+// number (weights are at most 1).
+struct PFp16 : Fp16 {
+    static constexpr int kBytes = 2, kBlocks = 2;
+    static constexpr float kPScale = 32768.f;
+    using T = uint16_t;
+    static __device__ __forceinline__ floatx4 mma16(vec8 a, vec8 b, floatx4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+};
+
+// ---- the schedule, found by every workgroup from the lengths
+struct PagedReq {
+    int start, len, t0, tiles;   // visible slots [start, len), key tiles [t0, t0 + tiles)
+};
+template <int TK>
+__device__ __forceinline__ PagedReq paged_req(const PagedAttnArgs &a, int b, bool report) {
+    PagedReq r{0, 0, 0, 0};
+    const int len = a.seq_len[b];
+    if (len < 0 || len > a.cap) {
+        if (report) raise_flag(a.status, CAST_FLAG_BAD_OFFSETS);
+        return r;
+    }
+    r.len = len;
+    r.start = a.window > 0 && len > a.window ? len - a.window : 0;
+    r.t0 = r.start / TK;
+    r.tiles = (len + TK - 1) / TK - r.t0;
+    return r;
+}
+
+// Tiles per split for the batch: an even share of the resident workgroups.
+template <int TK>
+__device__ __forceinline__ int paged_split(const PagedAttnArgs &a) {
+    if (a.split) return a.split;
+    const int lane = threadIdx.x & 63;
+    int64_t total = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 64)
+        total += p_wave_sum(b0 + lane < a.batch ? paged_req<TK>(a, b0 + lane, false).tiles : 0);
+    total *= a.Hkv * a.rbs;
+    const int64_t c = (total + a.slots - 1) / a.slots;
+    return c < kMinTiles ? kMinTiles : (int)c;
+}
+__device__ __forceinline__ int splits_of(int tiles, int split) {
+    return tiles <= split ? 1 : (int)(((uint32_t)tiles + (uint32_t)split - 1) / (uint32_t)split);
+}
+
+template <int D, typename E, bool PAD, bool ANY>
+__global__ __launch_bounds__(kPWaves * 64) void paged_attn_kernel(PagedAttnArgs a) {
+    using T = typename E::T;
+    constexpr bool F32 = E::kBytes == 4;
+    constexpr int KB = E::kBlocks;                 // 16-key blocks of a wave's tile
+    constexpr int WK = 16 * KB;                    // keys of a wave's tile
+    constexpr int TK = WK * kPWaves;               // keys of a workgroup's tile
+    constexpr int KC = F32 ? D / 16 : D / 32;      // 16-byte chunks of a key a lane holds (16 lanes hold a row's 4)
+    constexpr int EPC = F32 || D == 64 ? 4 : 8;    // elements of a V chunk
+    constexpr int VC = D / (16 * EPC);             // V chunks of a key a lane holds
+    constexpr int VK = 4 * KB;                     // keys a lane holds V of
+    constexpr int NA = D / 16;                     // 16-row blocks of O^T
+    constexpr int OP = D + 4;                      // row stride of the join's O (floats)
+    __shared__ __attribute__((aligned(16))) float Os[kPWaves][16][OP];
+    __shared__ float ML[kPWaves][16][2];
+
+    const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int dr = PAD ? a.D : D;
+
+    // ---- this workgroup's item: items run (request, split, query block, KV head), the head fastest
+    const int split = paged_split<TK>(a);
+    const int per = a.Hkv * a.rbs;
+    int b = 0, local = 0, first = 0;
+    {
+        int at = 0;
+        bool found = false;
+        for (int b0 = 0; b0 < a.batch && !found; b0 += 64) {
+            const int bb = b0 + lane;
+            const int n = bb < a.batch ? splits_of(paged_req<TK>(a, bb, blockIdx.x == 0 && w == 0).tiles, split) * per : 0;
+            const int incl = p_wave_scan(n);
+            const uint64_t past = __ballot(at + incl <= (int)blockIdx.x);
+            const int k = __popcll(past);
+            if (k < 64) {
+                found = true;
+                b = b0 + k;
+                first = at + __builtin_amdgcn_readlane(incl - n, k);
+                local = (int)blockIdx.x - first;
+            }
+            at += __builtin_amdgcn_readlane(incl, 63);
+        }
+        // (workgroup 0 finds its item in the first 64 requests; the rest are checked all the same)
+        if (blockIdx.x == 0 && w == 0)
+            for (int bb = 64 + lane; bb < a.batch; bb += 64) paged_req<TK>(a, bb, true);
+        if (!found || b >= a.batch) return;
+    }
+    const PagedReq rq = paged_req<TK>(a, b, false);
+    const int ns = splits_of(rq.tiles, split);
+    const int s = local / per, rest = local - s * per;
+    const int rb = rest / a.Hkv, h = rest - rb * a.Hkv;
+    if (ns > 1 && local == 0 && tid == 0) {
+        a.head[b] = first;
+        a.head[a.batch + b] = ns;
+    } else if (ns == 1 && a.head && local == 0 && tid == 0) {
+        a.head[a.batch + b] = 1;
+    }
+    // even splits: tiles [s, s + 1) * tiles / ns
+    const int ta = (int)((int64_t)rq.tiles * s / ns), tb = (int)((int64_t)rq.tiles * (s + 1) / ns);
+    const int nt = tb - ta;
+    const int key0 = (rq.t0 + ta) * TK + w * WK;   // the wave's first key
+    const int rows = min(16, a.G - rb * 16);       // query heads of this block
+    const int hq = h * a.G + rb * 16 + l16;
+
+    // ---- Q^T: head l16 of the block, chunks as K's
+    uint32_t qraw[KC][4];
+    {
+        const T *qp = static_cast<const T *>(a.q) + (int64_t)b * a.q_req + (int64_t)hq * a.q_head;
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+            const int d = F32 ? c * 16 + g * 4 : c * 32 + g * 8;
+            const bool in = l16 < rows && (!PAD || d < dr);
+            const u32x4 x = in ? *reinterpret_cast<const u32x4 *>(qp + d) : u32x4{};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) qraw[c][i] = x[i];
+        }
+    }
+    floatx4 acc[NA];
+#pragma unroll
+    for (int i = 0; i < NA; ++i) acc[i] = floatx4{};
+    float m = -INFINITY, l = 0.f;
+    bool bad = false, again = false;
+
+    // ---- page ids.  Without ANY a 16-key block lies within one page: lane
+    // 2 i + t (KB = 2) or i (KB = 1) holds the id of block t of tile i0 + i.
+    const char *kbase = static_cast<const char *>(a.k) + (int64_t)h * a.kp_head;
+    const char *vbase = static_cast<const char *>(a.v) + (int64_t)h * a.vp_head;
+    const int32_t *row = a.table + (int64_t)b * a.table_ld;
+    const uint32_t ps = (uint32_t)a.page_size;
+    auto seen = [&](int key) __attribute__((always_inline)) { return min(max(key, rq.start), rq.len - 1); };
+    auto page_id = [&](int key) __attribute__((always_inline)) {   // of a visible key; always a page of the pool
+        const int id = row[(uint32_t)key / ps];
+        bad |= id < 0 || id >= a.n_pages;
+        return min(max(id, 0), a.n_pages - 1);
+    };
+    int ids = 0;
+    auto load_ids = [&](int i0) __attribute__((always_inline)) {
+        const int i = min(i0 + lane / KB, nt - 1);
+        ids = page_id(seen(key0 + i * TK + (lane % KB) * 16));
+    };
+
+    struct Tile {
+        u32x4 k[KB][KC];
+        uint32_t v[VK][VC][EPC * E::kBytes / 4];
+    };
+    constexpr int VW = EPC * E::kBytes / 4;        // 32-bit words of a V chunk
+    auto load_tile = [&](Tile &t, int i) __attribute__((always_inline)) {
+        const int kt = key0 + i * TK;
+#pragma unroll
+        for (int t16 = 0; t16 < KB; ++t16) {
+            const int kb = kt + 16 * t16;
+            // this lane's K row, and the page and offset of its four V rows
+            const char *kp, *vp[4];
+            if constexpr (!ANY) {
+                // (visible keys of a block share a page; keys outside are clamped into them)
+                const int p0 = (int)((uint32_t)seen(kb) / ps * ps);
+                const int64_t id = __builtin_amdgcn_readlane(ids, (i % (64 / KB)) * KB + t16);
+                kp = kbase + id * a.kp_page + (int64_t)(seen(kb + l16) - p0) * a.kp_tok;
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    vp[r] = vbase + id * a.vp_page + (int64_t)(seen(kb + 4 * g + r) - p0) * a.vp_tok;
+            } else {
+                const int key = seen(kb + l16);
+                const int id = page_id(key), off = (int)((uint32_t)key % ps);
+                kp = kbase + (int64_t)id * a.kp_page + (int64_t)off * a.kp_tok;
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    vp[r] = vbase + (int64_t)__shfl(id, 4 * g + r) * a.vp_page + (int64_t)__shfl(off, 4 * g + r) * a.vp_tok;
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int c = 0; c < VC; ++c) {
+                    const int d = (c * 16 + l16) * EPC;
+                    const char *x = vp[r] + (PAD ? min(d, dr - EPC) : d) * E::kBytes;
+                    if constexpr (VW == 4) {
+                        const u32x4 y = *reinterpret_cast<const u32x4 *>(x);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) t.v[4 * t16 + r][c][e] = y[e];
+                    } else {
+                        const u32x2 y = *reinterpret_cast<const u32x2 *>(x);
+                        t.v[4 * t16 + r][c][0] = y[0];
+                        t.v[4 * t16 + r][c][1] = y[1];
+                    }
+                }
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+                const int d = F32 ? c * 16 + g * 4 : c * 32 + g * 8;
+                t.k[t16][c] = *reinterpret_cast<const u32x4 *>(kp + (PAD ? min(d, dr - 16 / E::kBytes) : d) * E::kBytes);
+            }
+        }
+    };
+
+    const float inv_cap = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
+    auto use_tile = [&](Tile &t, int i) __attribute__((always_inline)) {
+        const int kt = key0 + i * TK;
+        const bool edge = kt < rq.start || kt + WK > rq.len;
+        float p[KB][4];
+        // ---- scores, base 2
+#pragma unroll
+        for (int t16 = 0; t16 < KB; ++t16) {
+            floatx4 s4 = floatx4{};
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+                u32x4 kx = t.k[t16][c];
+                if constexpr (PAD) {
+                    // (chunks past the head dim were read from its last one)
+                    const int d = F32 ? c * 16 + g * 4 : c * 32 + g * 8;
+                    if (d >= dr) kx = u32x4{};
+                }
+                if constexpr (F32) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t kw = kx[e];   // (a bit cast of the element itself reads element 0)
+                        s4 = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, kw),
+                                                                  __builtin_bit_cast(float, qraw[c][e]), s4, 0, 0, 0);
+                    }
+                } else {
+                    const u32x4 qx = {qraw[c][0], qraw[c][1], qraw[c][2], qraw[c][3]};
+                    s4 = E::mma16(__builtin_bit_cast(typename E::vec8, kx), __builtin_bit_cast(typename E::vec8, qx), s4);
+                }
+            }
+            if (a.softcap > 0.f) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    // tanh: 1 - 2 / (e^2x + 1), near 0 (where that cancels) its
+                    // series to x^9, within 1e-8 of the value up to 1/4
+                    const float x = s4[r] * inv_cap, x2 = x * x;
+                    const float far = 1.f - 2.f / (__builtin_amdgcn_exp2f(x * (2.f * kPLog2e)) + 1.f);
+                    const float poly = fmaf(fmaf(fmaf(62.f / 2835.f, x2, -17.f / 315.f), x2, 2.f / 15.f), x2, -1.f / 3.f);
+                    const float near = fmaf(x * x2, poly, x);
+                    p[t16][r] = (x2 < 0.0625f ? near : far) * (a.softcap * kPLog2e);
+                }
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) p[t16][r] = s4[r] * a.scale;
+            }
+        }
+        if (edge) {
+#pragma unroll
+            for (int t16 = 0; t16 < KB; ++t16)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int key = kt + 16 * t16 + 4 * g + r;
+                    if (key < rq.start || key >= rq.len) {
+                        p[t16][r] = -INFINITY;
+#pragma unroll
+                        for (int c = 0; c < VC; ++c)
+#pragma unroll
+                            for (int e = 0; e < VW; ++e) t.v[4 * t16 + r][c][e] = 0u;
+                    }
+                }
+        }
+        // ---- running maximum: moved for all columns at once, when any needs it
+        float top = p[0][0];
+#pragma unroll
+        for (int t16 = 0; t16 < KB; ++t16)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) top = fmaxf(top, p[t16][r]);
+        if (__any(top > m)) {
+            const float mn = fmaxf(m, quad_max(top));
+            const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (int n = 0; n < NA; ++n) acc[n] *= alpha;
+        }
+        const float ms = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int t16 = 0; t16 < KB; ++t16)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                p[t16][r] = __builtin_amdgcn_exp2f(p[t16][r] - ms);
+                l += p[t16][r];
+            }
+        // ---- O^T += V^T P^T
+        if constexpr (F32) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int c = 0; c < VC; ++c)
+#pragma unroll
+                    for (int e = 0; e < EPC; ++e)
+                        acc[c * EPC + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, t.v[r][c][e]), p[0][r],
+                                                                                acc[c * EPC + e], 0, 0, 0);
+        } else {
+            u32x4 hi, lo;
+#pragma unroll
+            for (int t16 = 0; t16 < 2; ++t16)
+#pragma unroll
+                for (int r = 0; r < 4; r += 2) {
+                    const float x = p[t16][r] * E::kPScale, y = p[t16][r + 1] * E::kPScale;
+                    const uint32_t top2 = E::pack2(x, y);
+                    hi[2 * t16 + r / 2] = top2;
+                    lo[2 * t16 + r / 2] = E::pack2(x - E::widen((uint16_t)top2), y - E::widen((uint16_t)(top2 >> 16)));
+                }
+            if (again) {
+                // weights of one sign, none rounded to zero: infinities keep theirs
+#pragma unroll
+                for (int t16 = 0; t16 < 2; ++t16)
+#pragma unroll
+                    for (int r = 0; r < 4; r += 2) {
+                        const float x = p[t16][r], y = p[t16][r + 1];
+                        hi[2 * t16 + r / 2] = E::pack2(x > 0.f ? fmaxf(x, 0x1p-14f) : x, y > 0.f ? fmaxf(y, 0x1p-14f) : y);
+                    }
+                lo = hi;
+            }
+#pragma unroll
+            for (int c = 0; c < VC; ++c)
+#pragma unroll
+                for (int e = 0; e < EPC; ++e) {
+                    const uint32_t sel = (e & 1) ? 0x07060302u : 0x05040100u;
+                    u32x4 vx;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) vx[j] = __builtin_amdgcn_perm(t.v[2 * j + 1][c][e / 2], t.v[2 * j][c][e / 2], sel);
+                    const auto vv = __builtin_bit_cast(typename E::vec8, vx);
+                    acc[c * EPC + e] = E::mma16(vv, __builtin_bit_cast(typename E::vec8, hi), acc[c * EPC + e]);
+                    acc[c * EPC + e] = E::mma16(vv, __builtin_bit_cast(typename E::vec8, lo), acc[c * EPC + e]);
+                }
+        }
+    };
+
+    // where the wave's O^T lies in its part of the join's LDS
+    auto place = [&](int c, int r) __attribute__((always_inline)) { return &Os[w][l16][(c * 16 + 4 * g + r) * EPC]; };
+    if (nt > 0) {
+        for (;;) {
+            Tile buf[2];
+            if constexpr (!ANY) load_ids(0);
+            load_tile(buf[0], 0);
+            for (int i = 0; i < nt; i += 2) {
+                if (i + 1 < nt) load_tile(buf[1], i + 1);
+                use_tile(buf[0], i);
+                if (i + 1 >= nt) break;
+                if constexpr (!ANY)
+                    if ((i + 2) % (64 / KB) == 0) load_ids(i + 2);
+                if (i + 2 < nt) load_tile(buf[0], i + 2);
+                use_tile(buf[1], i + 1);
+            }
+            if (F32 || again) break;
+            // An infinite V times a weight's second term, of either sign or
+            // zero, is no number where infinity is meant: a wave whose sums
+            // are not all finite walks its keys again with weights of one
+            // sign, which decide only the elements that were not finite.
+            float z = 0.f;
+#pragma unroll
+            for (int n = 0; n < NA; ++n)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) z = fmaf(acc[n][r], 0.f, z);
+            if (!__any(l16 < rows && !(z == 0.f))) break;
+#pragma unroll
+            for (int c = 0; c < VC; ++c)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int e = 0; e < EPC; ++e) {
+                        place(c, r)[e] = acc[c * EPC + e][r];
+                        acc[c * EPC + e][r] = 0.f;
+                    }
+            m = -INFINITY;
+            l = 0.f;
+            again = true;
+        }
+    }
+
+    // ---- join the four waves
+    l = quad_sum(l);
+    const bool wbad = __any(bad);
+    if (l16 < rows) {
+#pragma unroll
+        for (int c = 0; c < VC; ++c)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int e = 0; e < EPC; ++e) {
+                    const float x = acc[c * EPC + e][r];
+                    if (!again || !(place(c, r)[e] * 0.f == 0.f)) place(c, r)[e] = x;
+                }
+    }
+    if (g == 0) {
+        ML[w][l16][0] = m;
+        ML[w][l16][1] = wbad ? -1.f : l;
+    }
+    __syncthreads();
+    const int quads = dr / 4;
+    for (int u = tid; u < rows * quads; u += kPWaves * 64) {
+        const int q = u / quads, d = (u - q * quads) * 4;
+        float mt = -INFINITY, lt = 0.f;
+        bool rejected = false;
+#pragma unroll
+        for (int x = 0; x < kPWaves; ++x) mt = fmaxf(mt, ML[x][q][0]);
+        const float ms = mt == -INFINITY ? 0.f : mt;
+        floatx4 o = floatx4{};
+#pragma unroll
+        for (int x = 0; x < kPWaves; ++x) {
+            const float f = __builtin_amdgcn_exp2f(ML[x][q][0] - ms), lx = ML[x][q][1];
+            rejected |= lx < 0.f;
+            lt = fmaf(lx, f, lt);
+            const floatx4 y = *reinterpret_cast<const floatx4 *>(&Os[x][q][d]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = fmaf(y[e], f, o[e]);
+        }
+        if (rejected && u == 0) raise_flag(a.status, CAST_FLAG_BAD_PAGE);
+        const int head = h * a.G + rb * 16 + q;
+        if (ns > 1) {
+            const int64_t at = (int64_t)blockIdx.x * 16 + q;
+            *reinterpret_cast<floatx4 *>(a.part_o + at * dr + d) = o;
+            if (d == 0) {
+                a.part_ml[at * 2] = mt;
+                a.part_ml[at * 2 + 1] = rejected ? -1.f : lt;
+            }
+        } else {
+            const float inv = rejected || lt == 0.f ? 0.f : 1.f / (lt * E::kPScale);
+            T *op = static_cast<T *>(a.out) + (int64_t)b * a.o_req + (int64_t)head * a.o_head + d;
+            if (rejected || lt == 0.f) o = floatx4{};
+            if constexpr (F32) {
+                *reinterpret_cast<floatx4 *>(op) = o * inv;
+            } else {
+                u32x2 y = {E::pack2(o[0] * inv, o[1] * inv), E::pack2(o[2] * inv, o[3] * inv)};
+                *reinterpret_cast<u32x2 *>(op) = y;
+            }
+            if (d == 0 && a.lse)
+                a.lse[(int64_t)b * a.Hq + head] = rejected || lt == 0.f ? -INFINITY : (ms + log2f(lt)) * kPLn2;
+        }
+    }
+}
+
+// Joins the splits of one (request, query head) per wave.
+template <typename E>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
+    using T = typename E::T;
+    const int b = blockIdx.y, lane = threadIdx.x & 63;
+    const int head = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (head >= a.Hq) return;
+    const int ns = a.head[a.batch + b];
+    if (ns <= 1) return;
+    const int h = head / a.G, in = head - h * a.G, rb = in / 16, q = in - rb * 16;
+    const int per = a.Hkv * a.rbs;
+    const int64_t item0 = (int64_t)a.head[b] + rb * a.Hkv + h;
+    float mt = -INFINITY;
+    bool rejected = false;
+    for (int s = lane; s < ns; s += 64) {
+        const float *ml = a.part_ml + ((item0 + (int64_t)s * per) * 16 + q) * 2;
+        mt = fmaxf(mt, ml[0]);
+        rejected |= ml[1] < 0.f;
+    }
+#pragma unroll
+    for (int off = 32; off; off >>= 1) mt = fmaxf(mt, __shfl_xor(mt, off));
+    rejected = __any(rejected);
+    const float ms = mt == -INFINITY ? 0.f : mt;
+    float lt = 0.f;
+    floatx4 o = floatx4{};
+    const int d = lane * 4;
+    for (int s0 = 0; s0 < ns; s0 += 64) {
+        float f = 0.f, lx = 0.f;
+        if (s0 + lane < ns) {
+            const float *ml = a.part_ml + ((item0 + (int64_t)(s0 + lane) * per) * 16 + q) * 2;
+            f = __builtin_amdgcn_exp2f(ml[0] - ms);
+            lx = ml[1] * f;
+        }
+        lt += lx;
+        const int n = min(64, ns - s0);
+        const float *po = a.part_o + ((item0 + (int64_t)s0 * per) * 16 + q) * a.D + min(d, a.D - 4);
+        const int64_t step = (int64_t)per * 16 * a.D;
+        for (int s1 = 0; s1 < n; s1 += 4) {
+            floatx4 y[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const floatx4 *>(po + min(s1 + j, n - 1) * step);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (s1 + j >= n) break;
+                const float fs = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), s1 + j));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = fmaf(y[j][e], fs, o[e]);
+            }
+        }
+    }
+#pragma unroll
+    for (int off = 32; off; off >>= 1) lt += __shfl_xor(lt, off);
+    const bool none = rejected || lt == 0.f;
+    const float inv = none ? 0.f : 1.f / (lt * E::kPScale);
+    if (none) o = floatx4{};
+    if (d < a.D) {
+        T *op = static_cast<T *>(a.out) + (int64_t)b * a.o_req + (int64_t)head * a.o_head + d;
+        if constexpr (E::kBytes == 4) {
+            *reinterpret_cast<floatx4 *>(op) = o * inv;
+        } else {
+            u32x2 y = {E::pack2(o[0] * inv, o[1] * inv), E::pack2(o[2] * inv, o[3] * inv)};
+            *reinterpret_cast<u32x2 *>(op) = y;
+        }
+    }
+    if (lane == 0 && a.lse) a.lse[(int64_t)b * a.Hq + head] = none ? -INFINITY : (ms + log2f(lt)) * kPLn2;
+}
+
+// --------------------------------------------------------------------------
+// Host side
+// --------------------------------------------------------------------------
+struct PagedKernel {
+    const void *fn;
+    int tile;   // keys of a workgroup's tile
+};
+template <int D, typename E, bool PAD, bool ANY>
+static PagedKernel paged_instance() {
+    return {reinterpret_cast<const void *>(&paged_attn_kernel<D, E, PAD, ANY>), 16 * E::kBlocks * kPWaves};
+}
+// Head dims 64, 128 and 256 have instances of their own; other multiples of 8
+// take the next larger one with the rest masked.  Page sizes whose 16-key
+// blocks may straddle a page take the instances that look up every key.
+template <int D, typename E>
+static PagedKernel paged_instance_of(bool pad, bool any) {
+    if (any) return paged_instance<D, E, true, true>();
+    return pad ? paged_instance<D, E, true, false>() : paged_instance<D, E, false, false>();
+}
+template <typename E>
+static PagedKernel paged_kernel_of(int32_t D, bool any) {
+    if (D <= 64) return paged_instance_of<64, E>(D != 64, any);
+    if (D <= 128) return paged_instance_of<128, E>(D != 128, any);
+    return paged_instance_of<256, E>(D != 256, any);
+}
+static PagedKernel paged_kernel(int32_t dtype, int32_t D, bool any) {
+    if (dtype == CAST_FP32) return paged_kernel_of<PF32>(D, any);
+    return dtype == CAST_FP16 ? paged_kernel_of<PFp16>(D, any) : paged_kernel_of<PBf16>(D, any);
+}
+static bool paged_any(int32_t page_size, int32_t max_pages) { return page_size % 16 != 0 && max_pages > 1; }
+
+// Workgroups of kernel k that the current device holds at once (an MI355X's
+// 256 CUs, one each, where no device is visible), looked up once per (device,
+// kernel).
+static int paged_slots(const PagedKernel &k) {
+    struct Entry {
+        int dev;
+        const void *fn;
+        int n;
+    };
+    static std::mutex mu;
+    static Entry cache[128];
+    static int used = 0;
+    int dev = -1;
+    if (hipGetDevice(&dev) != hipSuccess) return 256;
+    std::lock_guard<std::mutex> lock(mu);
+    for (int i = 0; i < used; ++i)
+        if (cache[i].dev == dev && cache[i].fn == k.fn) return cache[i].n;
+    int n = 0, cus = 0;
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, k.fn, kPWaves * 64, 0) != hipSuccess || n < 1) n = 1;
+    if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus < 1) cus = 256;
+    n *= cus;
+    if (used < 128) cache[used++] = Entry{dev, k.fn, n};
+    return n;
+}
+
+struct PagedPlan {
+    int32_t split;      // as PagedAttnArgs
+    int32_t slots;
+    int64_t items;      // workgroups, an upper bound for any lengths
+    bool parts;         // whether a request may be split
+};
+static PagedPlan paged_plan(int32_t batch, int32_t max_pages, int32_t page_size, int32_t Hq, int32_t Hkv, int32_t D,
+                            int32_t window, int32_t dtype, int32_t kv_split) {
+    const PagedKernel k = paged_kernel(dtype, D, paged_any(page_size, max_pages));
+    PagedPlan p{};
+    p.slots = paged_slots(k);
+    const int64_t per = (int64_t)Hkv * ((Hq / Hkv + 15) / 16);
+    int64_t keys = (int64_t)max_pages * page_size;
+    if (window > 0 && window < keys) keys = (int64_t)window + k.tile - 1;   // (a window may start inside a tile)
+    const int64_t tiles = (keys + k.tile - 1) / k.tile;
+    int64_t least = kMinTiles;
+    if (kv_split > 0) {
+        p.split = (int32_t)(((int64_t)kv_split + k.tile - 1) / k.tile);
+        least = p.split;
+    } else if (kv_split < 0) {
+        p.split = INT_MAX;
+        least = INT_MAX;
+    }
+    const int64_t most = tiles <= least ? 1 : (tiles + least - 1) / least;   // splits of one request
+    p.parts = most > 1;
+    if (!p.parts) p.split = INT_MAX;
+    p.items = batch * per * most;
+    // an automatic split of c tiles, c * slots >= all tiles, makes at most
+    // slots + one item per unit
+    if (kv_split == 0 && p.parts && p.items > p.slots + batch * per) p.items = p.slots + batch * per;
+    return p;
+}
+static size_t p_align256(size_t x) { return (x + 255) & ~(size_t)255; }
+static size_t paged_ws(const PagedPlan &p, int32_t batch, int32_t D) {
+    if (!p.parts) return 0;
+    return p_align256((size_t)batch * 2 * sizeof(int32_t)) + p_align256((size_t)p.items * 16 * 2 * sizeof(float)) +
+           p_align256((size_t)p.items * 16 * D * sizeof(float));
+}
+
+}  // namespace cast
+
+using namespace cast;
+
+extern "C" size_t cast_paged_attn_workspace_size(int32_t batch, int32_t max_pages, int32_t page_size,
+                                                 int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                                                 int32_t window, int32_t dtype, int32_t kv_split) {
+    if (batch <= 0 || max_pages <= 0 || page_size <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
+        num_q_heads % num_kv_heads || head_dim <= 0 || head_dim % 8 || head_dim > 256)
+        return 0;
+    if (dtype != CAST_BF16 && dtype != CAST_FP16 && dtype != CAST_FP32) return 0;
+    return paged_ws(paged_plan(batch, max_pages, page_size, num_q_heads, num_kv_heads, head_dim, window, dtype, kv_split),
+                    batch, head_dim);
+}
+
+extern "C" int cast_paged_attn_fwd(const void *q, const void *k_pages, const void *v_pages, void *out, float *lse,
+                                   const int32_t *page_table, int64_t table_ld, int32_t max_pages, int32_t n_pages,
+                                   int32_t page_size, const int32_t *seq_len, int32_t batch, int32_t num_q_heads,
+                                   int32_t num_kv_heads, int32_t head_dim, int64_t q_req, int64_t q_head,
+                                   int64_t kp_page, int64_t kp_head, int64_t kp_tok, int64_t vp_page, int64_t vp_head,
+                                   int64_t vp_tok, int64_t o_req, int64_t o_head, int32_t dtype, float sm_scale,
+                                   float softcap, int32_t window, int32_t kv_split, void *workspace,
+                                   size_t workspace_bytes, int32_t *status, cast_stream_t stream) {
+    if (batch < 0 || max_pages < 0 || n_pages < 0 || page_size <= 0 || window < 0 || head_dim <= 0) return CAST_ERR_SHAPE;
+    if (num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads) return CAST_ERR_HEAD_RATIO;
+    if (dtype != CAST_BF16 && dtype != CAST_FP16 && dtype != CAST_FP32) return CAST_ERR_DTYPE;
+    if (head_dim % 8 || head_dim > 256) return CAST_ERR_HEAD_DIM;
+    if (!(sm_scale > 0.f) || !isfinite(sm_scale) || !(softcap >= 0.f) || !isfinite(softcap)) return CAST_ERR_SCALE;
+    if (batch == 0) return CAST_OK;
+    // every request's visible keys need a page to be read from
+    if (max_pages == 0 || n_pages == 0) return CAST_ERR_SHAPE;
+    if ((int64_t)max_pages * page_size > INT32_MAX - 512) return CAST_ERR_SHAPE;
+    if (!q || !k_pages || !v_pages || !out || !page_table || !seq_len) return CAST_ERR_NULL_POINTER;
+    const int64_t esz = dtype == CAST_FP32 ? 4 : 2;
+    auto a16 = [](const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+    if (!a16(q) || !a16(k_pages) || !a16(v_pages) || !a16(out)) return CAST_ERR_ALIGNMENT;
+    const int64_t strides[10] = {q_req, q_head, kp_page, kp_head, kp_tok, vp_page, vp_head, vp_tok, o_req, o_head};
+    for (int64_t s : strides)
+        if ((s * esz) % 16) return CAST_ERR_ALIGNMENT;
+    const bool any = paged_any(page_size, max_pages);
+    const PagedPlan p = paged_plan(batch, max_pages, page_size, num_q_heads, num_kv_heads, head_dim, window, dtype, kv_split);
+    if (p.items > INT32_MAX || batch > 65535) return CAST_ERR_SHAPE;
+    if (p.parts) {
+        if (!workspace) return CAST_ERR_NULL_POINTER;
+        if (workspace_bytes < paged_ws(p, batch, head_dim)) return CAST_ERR_WORKSPACE;
+        if (reinterpret_cast<uintptr_t>(workspace) & 255) return CAST_ERR_ALIGNMENT;
+    }
+    PagedAttnArgs a{};
+    a.q = q;
+    a.k = k_pages;
+    a.v = v_pages;
+    a.out = out;
+    a.lse = lse;
+    a.table = page_table;
+    a.seq_len = seq_len;
+    a.status = status;
+    a.table_ld = table_ld;
+    a.q_req = q_req;
+    a.q_head = q_head;
+    a.o_req = o_req;
+    a.o_head = o_head;
+    a.kp_page = kp_page * esz;
+    a.kp_head = kp_head * esz;
+    a.kp_tok = kp_tok * esz;
+    a.vp_page = vp_page * esz;
+    a.vp_head = vp_head * esz;
+    a.vp_tok = vp_tok * esz;
+    a.n_pages = n_pages;
+    a.page_size = page_size;
+    a.batch = batch;
+    a.Hq = num_q_heads;
+    a.Hkv = num_kv_heads;
+    a.G = num_q_heads / num_kv_heads;
+    a.rbs = (a.G + 15) / 16;
+    a.D = head_dim;
+    a.cap = max_pages * page_size;
+    a.window = window;
+    a.split = p.split;
+    a.slots = p.slots;
+    a.softcap = softcap;
+    a.scale = softcap > 0.f ? sm_scale : sm_scale * kPLog2e;
+    if (p.parts) {
+        char *ws = static_cast<char *>(workspace);
+        a.head = reinterpret_cast<int32_t *>(ws);
+        ws += p_align256((size_t)batch * 2 * sizeof(int32_t));
+        a.part_ml = reinterpret_cast<float *>(ws);
+        ws += p_align256((size_t)p.items * 16 * 2 * sizeof(float));
+        a.part_o = reinterpret_cast<float *>(ws);
+    }
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    void *args[] = {&a};
+    const PagedKernel k = paged_kernel(dtype, head_dim, any);
+    if (hipLaunchKernel(k.fn, dim3((unsigned)p.items), dim3(kPWaves * 64), args, 0, st) != hipSuccess) return CAST_ERR_HIP;
+    if (p.parts) {
+        const dim3 grid((unsigned)((num_q_heads + 3) / 4), (unsigned)batch);
+        if (dtype == CAST_FP32) paged_join_kernel<PF32><<<grid, 256, 0, st>>>(a);
+        else if (dtype == CAST_FP16) paged_join_kernel<PFp16><<<grid, 256, 0, st>>>(a);
+        else paged_join_kernel<PBf16><<<grid, 256, 0, st>>>(a);
+        if (hipGetLastError() != hipSuccess) return CAST_ERR_HIP;
+    }
+    return CAST_OK;
+}

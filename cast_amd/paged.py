@@ -1,0 +1,261 @@
+"""A KV cache of pages: append with the rotation on the way, and the attention
+of one new token per request (HIP, gfx950).
+
+  paged_append     rows of new K and V into their requests' pages, K (and Q)
+                   rotated to their positions by cos / sin tables; the paged
+                   form of cast_trees/serving.py:264-289
+  paged_attention  one query token per request against the pages: the ordinary
+                   decode step (cast_trees/decode.py:211-231 runs it inside the
+                   model) beside the tree verification
+
+A layer's pool is ``[n_pages, Hkv, page_size, D]`` in bfloat16, float16 or
+float32, with any strides of its first three dimensions that keep rows 16-byte
+aligned (a ``[n_pages, page_size, Hkv, D]`` cache is passed as
+``pool.transpose(1, 2)``).  Slot t of request b lies in page ``page_table[b, t
+// page_size]`` at offset ``t % page_size``; ``page_table`` is int32 ``[B,
+max_pages]``, entries behind a request's last page may be anything.  The
+per-request store ``[B, Hkv, cap, D]`` of ``cast_amd.serving`` is such a pool of
+one page per request: ``page_table = arange(B)[:, None]``.
+
+Everything is stream-ordered on torch's current stream; nothing synchronises
+unless ``check=True``, which reads the device status word once and raises
+``ValueError``.
+"""
+from __future__ import annotations
+
+import ctypes
+import functools
+import math
+import operator
+
+import torch
+
+from . import _lib
+from .tree_attn import _DTYPES, _as_i32, _ready, _require_on
+
+
+def _pools(k_pages, v_pages, what):
+    """The pools' common geometry (n_pages, Hkv, page_size, D)."""
+    if k_pages.dim() != 4 or tuple(v_pages.shape) != tuple(k_pages.shape):
+        raise ValueError("k_pages and v_pages must both be [n_pages, H_kv, page_size, D]")
+    if not k_pages.is_cuda:
+        raise ValueError(f"{what} runs on the GPU: the pools must be device tensors")
+    if k_pages.dtype not in _DTYPES or v_pages.dtype != k_pages.dtype:
+        raise ValueError("the pools must share one dtype: bfloat16, float16 or float32")
+    esz = k_pages.element_size()
+    if not (_in_place(k_pages, esz) and _in_place(v_pages, esz)):
+        raise ValueError("the pools need a contiguous head dim and 16-byte aligned strides")
+    return (int(x) for x in k_pages.shape)
+
+
+def _table(page_table, dev, batch=None):
+    """page_table as int32 rows on dev (no copy when it already is that)."""
+    t = page_table
+    if not (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.get_device() == dev.index
+            and t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] <= 1)):
+        t = _as_i32(t, dev)
+    if t.dim() != 2 or (batch is not None and t.shape[0] != batch):
+        raise ValueError("page_table must be [B, max_pages]")
+    return t
+
+
+def _in_place(x, esz):
+    """Whether the kernels can address x as it lies: head dim contiguous, 16-byte aligned base and strides."""
+    return x.numel() == 0 or (_ready(x, esz) is x and not x.data_ptr() & 15)
+
+
+def _aligned(x, esz):
+    """x, or a copy the kernels can address."""
+    return x if _in_place(x, esz) else x.clone(memory_format=torch.contiguous_format)
+
+
+def _no_overlap(name, t):
+    """An output whose elements share memory (an expanded tensor) cannot be written."""
+    if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+        raise ValueError(f"{name} must not be an expanded tensor")
+
+
+def _rows(name, x, heads, D, dtype, total=None):
+    if x.dim() != 3 or x.shape[1:] != (heads, D) or (total is not None and x.shape[0] != total):
+        raise ValueError(f"{name} must be [{'total' if total is None else total}, {heads}, {D}]")
+    if x.dtype != dtype:
+        raise ValueError(f"{name} must have the pools' dtype {dtype}")
+
+
+def paged_append(k, v, k_pages, v_pages, page_table, seq_len, cu_q=None, *, q=None, cos=None, sin=None,
+                 positions=None, interleaved=False, q_out=None, k_out=None, new_len=None, check=False):
+    """Write new tokens into the cache; returns ``(q_rotated, new_len)``.
+
+    k / v: [total, H_kv, D] rows of the new tokens (any token and head
+    strides); seq_len int32 [B]: tokens of each request already in the cache.
+    Request b appends rows cu_q[b] .. cu_q[b + 1] - 1 (``cu_q=None``: one token
+    each, row b) to slots seq_len[b], seq_len[b] + 1, ...  ``new_len`` int32 [B]
+    (allocated unless given) is seq_len plus the rows appended.
+
+    cos / sin: float32 [max_pos, rot_dim / 2]; with them the first rot_dim
+    elements of every K head are rotated before they are stored: element pairs
+    (i, i + rot_dim / 2), or (2i, 2i + 1) with ``interleaved``, by the angle of
+    the token's slot or of ``positions`` int32 [total].  rot_dim: a multiple of
+    16 (float32: of 8).  ``q`` [total, H_q, D] is rotated alike into ``q_out``
+    (allocated unless given; may be q itself); without tables it is copied.
+    ``k_out`` also receives the rotated K (may be k itself).
+
+    A row with an invalid slot, page id or position is skipped whole, and its
+    request's new_len stays seq_len; ``check=True`` raises.
+    """
+    lib = _lib.load()
+    n_pages, H_kv, page_size, D = _pools(k_pages, v_pages, "paged_append")
+    dt, dev = k_pages.dtype, k_pages.device
+    _rows("k", k, H_kv, D, dt)
+    total = int(k.shape[0])
+    _rows("v", v, H_kv, D, dt, total)
+    _require_on(dev, v_pages=v_pages, k=k, v=v, q=q, cos=cos, sin=sin, q_out=q_out, k_out=k_out, new_len=new_len)
+    esz = k.element_size()
+    H_q = 0
+    if q is not None:
+        H_q = int(q.shape[1]) if q.dim() == 3 else 0
+        _rows("q", q, H_q, D, dt, total)
+        assert H_q > 0 and H_q % H_kv == 0
+        if q_out is None:
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    for name, t, heads in (("q_out", q_out, H_q), ("k_out", k_out, H_kv)):
+        if t is not None:
+            _rows(name, t, heads, D, dt, total)
+            _no_overlap(name, t)
+            if not _in_place(t, esz):
+                raise ValueError(f"{name} needs a contiguous head dim and 16-byte aligned strides")
+    k, v = _aligned(k, esz), _aligned(v, esz)
+    q = None if q is None else _aligned(q, esz)
+    rot_dim = max_pos = rope_ld = 0
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin go together")
+    if cos is not None:
+        if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+            raise ValueError("cos and sin must both be float32 [max_pos, rot_dim / 2]")
+        max_pos, rot_dim = int(cos.shape[0]), 2 * int(cos.shape[1])
+        if not 0 < rot_dim <= D or rot_dim % (32 // esz):
+            raise ValueError(f"rot_dim must be a multiple of {32 // esz} up to the head dim {D}, got {rot_dim}")
+        cos, sin = _aligned(cos, 4), _aligned(sin, 4)
+        if cos.stride() != sin.stride():
+            cos, sin = cos.contiguous(), sin.contiguous()
+        rope_ld = cos.stride(0) if max_pos > 1 else rot_dim // 2
+        if positions is not None:
+            positions = _as_i32(positions, dev)
+            if positions.shape != (total,):
+                raise ValueError(f"positions must be [{total}]")
+    else:
+        positions = None
+    page_table = _table(page_table, dev)
+    seq_len = _as_i32(seq_len, dev)
+    B, max_pages = (int(x) for x in page_table.shape)
+    if seq_len.shape != (B,):
+        raise ValueError(f"seq_len must be [{B}], one entry per page_table row")
+    if cu_q is not None:
+        cu_q = _as_i32(cu_q, dev)
+        if cu_q.shape != (B + 1,):
+            raise ValueError("cu_q needs B+1 entries")
+    elif total != B:
+        raise ValueError("without cu_q every request appends one row: k must have B rows")
+    if new_len is None:
+        new_len = torch.empty_like(seq_len)
+    elif new_len.dtype != torch.int32 or new_len.shape != (B,) or not new_len.is_contiguous():
+        raise ValueError(f"new_len must be a contiguous int32 [{B}]")
+    status = torch.zeros(1, dtype=torch.int32, device=dev) if check else None
+    one = lambda t: (ctypes.c_void_p * 1)(t.data_ptr())
+    qs, qo, ko = (t.stride()[:2] if t is not None else (0, 0) for t in (q, q_out, k_out))
+    if total or B:
+        with _lib.on_device(dev):
+            st = lib.cast_paged_append(
+                one(k), one(v), one(k_pages), one(v_pages), 1 if total else 0, page_table.data_ptr(),
+                page_table.stride(0), max_pages, n_pages, page_size, seq_len.data_ptr(), new_len.data_ptr(), B, total,
+                _lib.ptr(cu_q), None, 0, None, _lib.ptr(q), _lib.ptr(q_out), _lib.ptr(k_out), _lib.ptr(cos),
+                _lib.ptr(sin), rope_ld, max_pos, rot_dim, int(bool(interleaved)), _lib.ptr(positions), H_q, H_kv, D,
+                *k.stride()[:2], *v.stride()[:2], *k_pages.stride()[:3], *v_pages.stride()[:3], *qs, *qo, *ko,
+                _DTYPES[dt], _lib.ptr(status), _lib.stream_of(k_pages))
+        _lib.check(st, "cast_paged_append")
+    if not total:
+        new_len.copy_(seq_len)      # nothing to append
+    if check:
+        _lib.raise_device_flags(status.item(), "paged_append")
+    return q_out, new_len
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(device_index, *sizes):
+    """cast_paged_attn_workspace_size of one call's sizes, asked once per size
+    with the device current (plain ints: a function of them alone)."""
+    with _lib.on_device(torch.device("cuda", device_index)):
+        return _lib.load().cast_paged_attn_workspace_size(*sizes)
+
+
+def paged_attention(q, k_pages, v_pages, page_table, seq_len, sm_scale=None, *, softcap=0.0, window=0,
+                    return_lse=False, kv_split=0, check=False, out=None, workspace=None):
+    """q: [B, H_q, D], one new token per request -> [B, H_q, D].
+
+    seq_len int32 [B]: slots request b's query sees, its own token's included
+    (0 gives zeros and lse = -inf).  Scores are ``sm_scale * q.k`` (default
+    1 / sqrt(D)), capped to ``softcap * tanh(score / softcap)`` when softcap is
+    positive; with ``window > 0`` only the last ``window`` slots are seen.
+    ``return_lse`` also returns their natural-log log-sum-exp [B, H_q] (fp32).
+    ``kv_split``: keys per split of a request (0: chosen on the device from the
+    lengths; negative: no split).  ``workspace``: uint8 device tensor of at
+    least ``paged_workspace_bytes(...)``; one is allocated when missing or too
+    small.  Calls that share a workspace must not overlap.
+
+    Requests with a length outside the table or a visible page id outside the
+    pool return zeros with lse = -inf; ``check=True`` raises.
+    """
+    lib = _lib.load()
+    kv_split, window = operator.index(kv_split), operator.index(window)
+    n_pages, H_kv, page_size, D = _pools(k_pages, v_pages, "paged_attention")
+    if q.dim() != 3 or q.shape[2] != D:
+        raise ValueError(f"q must be [B, H_q, {D}], the pools' head dim")
+    B, H_q = int(q.shape[0]), int(q.shape[1])
+    assert H_q % H_kv == 0
+    if q.dtype != k_pages.dtype:
+        raise ValueError("q and the pools must share one dtype (the cache is read in place)")
+    dev = k_pages.device
+    _require_on(dev, q=q, v_pages=v_pages, out=out, workspace=workspace)
+    if window < 0 or softcap is None or not (0 <= softcap < math.inf):
+        raise ValueError("window and softcap must be 0 (none) or positive")
+    esz = q.element_size()
+    q = _aligned(q, esz)
+    page_table = _table(page_table, dev, B)
+    seq_len = _as_i32(seq_len, dev)
+    if seq_len.shape != (B,):
+        raise ValueError(f"seq_len must be [{B}]")
+    if out is None:
+        out = q.new_empty((B, H_q, D))
+    else:
+        if out.shape != q.shape or out.dtype != q.dtype or not _in_place(out, esz):
+            raise ValueError("out must match q's shape and dtype with a contiguous head dim, 16-byte aligned")
+        _no_overlap("out", out)
+    lse = q.new_empty((B, H_q), dtype=torch.float32) if return_lse else None
+    if sm_scale is None:
+        sm_scale = 1.0 / math.sqrt(D)
+    max_pages = int(page_table.shape[1])
+    dt = _DTYPES[q.dtype]
+    status = torch.zeros(1, dtype=torch.int32, device=dev) if check else None
+    ws_bytes = _workspace_bytes(dev.index, B, max_pages, page_size, H_q, H_kv, D, window, dt, kv_split)
+    if ws_bytes and (workspace is None or workspace.numel() * workspace.element_size() < ws_bytes):
+        workspace = q.new_empty(ws_bytes, dtype=torch.uint8)
+    with _lib.on_device(dev):
+        st = lib.cast_paged_attn_fwd(
+            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), _lib.ptr(lse), page_table.data_ptr(),
+            page_table.stride(0), max_pages, n_pages, page_size, seq_len.data_ptr(), B, H_q, H_kv, D, *q.stride()[:2],
+            *k_pages.stride()[:3], *v_pages.stride()[:3], *out.stride()[:2], dt, float(sm_scale), float(softcap),
+            window, kv_split, _lib.ptr(workspace) if ws_bytes else None, ws_bytes, _lib.ptr(status),
+            _lib.stream_of(q))
+    _lib.check(st, "cast_paged_attn_fwd")
+    if check:
+        _lib.raise_device_flags(status.item(), "paged_attention")
+    return (out, lse) if return_lse else out
+
+
+def paged_workspace_bytes(batch, max_pages, page_size, H_q, H_kv, D, dtype=torch.bfloat16, window=0, kv_split=0,
+                          device=None):
+    """Bytes of split workspace one ``paged_attention`` call of these sizes needs."""
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    return _workspace_bytes(dev.index or 0, batch, max_pages, page_size, H_q, H_kv, D, window, _DTYPES[dtype], kv_split)

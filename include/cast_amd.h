@@ -51,9 +51,11 @@ enum cast_device_flag {
     CAST_FLAG_BAD_PACK = 1,        /* pack_len outside [1, 128] or beyond the mask words */
     CAST_FLAG_BAD_OFFSETS = 2,     /* cu_q / cu_kv / prefix_len inconsistent with totals */
     CAST_FLAG_BAD_PARENT = 4,      /* a parent index not in [-1, own index) */
-    CAST_FLAG_TOO_LONG = 8         /* a request's key source exceeds the kernel's
+    CAST_FLAG_TOO_LONG = 8,        /* a request's key source exceeds the kernel's
                                       row addressing (bf16 MFMA path: 2^24 - 64
                                       rows and 2^31 bytes per source) */
+    CAST_FLAG_BAD_PAGE = 16,       /* a page id outside [0, n_pages) */
+    CAST_FLAG_BAD_POSITION = 32    /* a position outside the rotation tables */
 };
 
 enum cast_dtype { CAST_BF16 = 0, CAST_FP32 = 1, CAST_FP64 = 2, CAST_FP16 = 3 };
@@ -359,6 +361,102 @@ int cast_build_trees_uniform(const int64_t *top_idx, const void *top_lp, int32_t
                              int32_t batch, int32_t L, int32_t k, int32_t nodes, int64_t *token,
                              int32_t *depth, int32_t *parent, double *score, int32_t *n_nodes,
                              int32_t *status, cast_stream_t stream);
+
+/* ---------------------------------------------------------------------
+ * A KV cache of pages.  The pool of each layer is [n_pages, Hkv, page_size,
+ * D] in any strides of its first three dimensions (in elements; 16-byte
+ * aligned, the head dim contiguous), and slot t of request b lies in page
+ * page_table[b * table_ld + t / page_size] at offset t % page_size; a table
+ * row covers max_pages * page_size < 2^31 slots.  A store [B, Hkv, cap, D]
+ * (cast_trees/serving.py:191-205) is such a pool of one page of cap slots per
+ * request.  Page ids are checked on the device wherever they are used.
+ * ------------------------------------------------------------------- */
+
+/* ---------------------------------------------------------------------
+ * K6: rows of new K and V into the pages, K (and Q) rotated on the way.
+ * The paged form of _append_store (cast_trees/serving.py:264-289), and the
+ * append of an ordinary decode step or a prompt.
+ *   k, v            HOST arrays of `layers` device pointers to the new rows
+ *                   [total, Hkv, D] (strides k_* / v_*)
+ *   k_pages/v_pages HOST arrays of `layers` device pointers to the pools
+ *   seq_len  int32 [batch]    tokens of each request already in the cache
+ *   new_len  int32 [batch]    out (nullable): seq_len + rows appended; for a
+ *                   request with a row that cannot be placed seq_len, so that
+ *                   none of its new slots is seen.  It must not overlap
+ *                   an input that other workgroups still read (CAST_ERR_ALIAS)
+ *   cu_q     int32 [batch+1]  request b appends packed rows [cu_q[b],
+ *                   cu_q[b+1]); NULL: row b alone.  Rows outside every
+ *                   request are left alone
+ *   path, path_len  (nullable) accepted nodes as cast_greedy_accept writes
+ *                   them: request b appends its root, row cu_q[b], and rows
+ *                   cu_q[b] + 1 + path[b][j], j < path_len[b]
+ *   q, q_out        (nullable) [total, Hq, D]: rotated like K; q_out may be q
+ *   k_out           (nullable) [total, Hkv, D]: the rotated K; may be k
+ *   cos, sin        (nullable) float [max_pos][rot_dim / 2], rows rope_ld
+ *                   elements apart (a multiple of 4): pairs (x, y) of the
+ *                   first rot_dim elements become (x cos - y sin, y cos +
+ *                   x sin), computed in float and rounded once.  Pair i is
+ *                   elements (i, i + rot_dim / 2), interleaved != 0:
+ *                   (2i, 2i + 1).  rot_dim a multiple of 16 (fp32: 8)
+ *   positions int32 [total]   (nullable) the tables' row of each token; NULL:
+ *                   its slot
+ * Rotation, q and k_out take one layer and no path.  A row whose slot, page
+ * id or position is out of range is skipped whole (its pages, q_out and
+ * k_out rows keep what they held); *status gets CAST_FLAG_BAD_OFFSETS,
+ * _BAD_PAGE or _BAD_POSITION.  Two rows that the tables send to one slot
+ * leave either's elements.
+ * ------------------------------------------------------------------- */
+int cast_paged_append(const void *const *k, const void *const *v, void *const *k_pages,
+                      void *const *v_pages, int32_t layers, const int32_t *page_table,
+                      int64_t table_ld, int32_t max_pages, int32_t n_pages, int32_t page_size,
+                      const int32_t *seq_len, int32_t *new_len, int32_t batch, int32_t total,
+                      const int32_t *cu_q, const int32_t *path, int32_t path_stride,
+                      const int32_t *path_len, const void *q, void *q_out, void *k_out,
+                      const float *cos, const float *sin, int64_t rope_ld, int32_t max_pos,
+                      int32_t rot_dim, int32_t interleaved, const int32_t *positions,
+                      int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int64_t k_tok,
+                      int64_t k_head, int64_t v_tok, int64_t v_head, int64_t kp_page,
+                      int64_t kp_head, int64_t kp_tok, int64_t vp_page, int64_t vp_head,
+                      int64_t vp_tok, int64_t q_tok, int64_t q_head, int64_t qo_tok,
+                      int64_t qo_head, int64_t ko_tok, int64_t ko_head, int32_t dtype,
+                      int32_t *status, cast_stream_t stream);
+
+/* ---------------------------------------------------------------------
+ * K7: attention of one new token per request over the pages, the decode
+ * step beside the tree verification (the attention inside
+ * cast_trees/decode.py:211-231 ar_generate's model step).
+ *   q        [batch, Hq, D] strides (q_req, q_head, 1); out likewise (o_*)
+ *   lse      float [batch, Hq] (nullable), natural log-sum-exp of the scores
+ *   seq_len  int32 [batch]  slots that request b's query sees, its own token's
+ *            included (0: zeros, lse = -inf)
+ *   softcap  > 0: scores become softcap * tanh(score / softcap); 0: none
+ *   window   > 0: only the last `window` slots are seen; 0: all.  Pages in
+ *            front of the window are not looked up
+ *   head_dim any multiple of 8 up to 256; dtypes CAST_BF16, _FP16, _FP32
+ *   kv_split keys per split (rounded up to key tiles of 128, fp32 64); 0: an
+ *            even share of the workgroups the device holds, from the lengths;
+ *            negative: one split
+ *   workspace  cast_paged_attn_workspace_size(...) bytes, 256-byte aligned
+ *            (may be NULL when that is 0); calls sharing one must not overlap
+ * A request whose seq_len is outside [0, max_pages * page_size]
+ * (CAST_FLAG_BAD_OFFSETS) or that sees a page id outside [0, n_pages)
+ * (CAST_FLAG_BAD_PAGE) gets zeros and lse = -inf.  Slots it does not see may
+ * hold anything.  batch at most 65535.
+ * ------------------------------------------------------------------- */
+int cast_paged_attn_fwd(const void *q, const void *k_pages, const void *v_pages, void *out,
+                        float *lse, const int32_t *page_table, int64_t table_ld,
+                        int32_t max_pages, int32_t n_pages, int32_t page_size,
+                        const int32_t *seq_len, int32_t batch, int32_t num_q_heads,
+                        int32_t num_kv_heads, int32_t head_dim, int64_t q_req, int64_t q_head,
+                        int64_t kp_page, int64_t kp_head, int64_t kp_tok, int64_t vp_page,
+                        int64_t vp_head, int64_t vp_tok, int64_t o_req, int64_t o_head,
+                        int32_t dtype, float sm_scale, float softcap, int32_t window,
+                        int32_t kv_split, void *workspace, size_t workspace_bytes,
+                        int32_t *status, cast_stream_t stream);
+size_t cast_paged_attn_workspace_size(int32_t batch, int32_t max_pages, int32_t page_size,
+                                      int32_t num_q_heads, int32_t num_kv_heads,
+                                      int32_t head_dim, int32_t window, int32_t dtype,
+                                      int32_t kv_split);
 
 
 #ifdef __cplusplus
