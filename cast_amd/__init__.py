@@ -31,7 +31,9 @@ _LAZY = {
     "build_trees": "draft",
     "paged_append": "paged",
     "paged_attention": "paged",
+    "paged_tree_attention": "paged",
     "paged_workspace_bytes": "paged",
+    "paged_tree_workspace_bytes": "paged",
     "build_tree_device": "draft",
 }
 

@@ -57,6 +57,9 @@ SIGNATURES = {
     "cast_paged_attn_fwd": ([_P] * 6 + [_I64, _I32, _I32, _I32, _P, _I32, _I32, _I32, _I32] + [_I64] * 10 +
                             [_I32, ctypes.c_float, ctypes.c_float, _I32, _I32, _P, _SZ, _P, _P], ctypes.c_int),
     "cast_paged_attn_workspace_size": ([_I32] * 9, _SZ),
+    "cast_tree_attn_paged_fwd": ([_P] * 4 + [_I64, _I32, _I32, _I32] + [_P] * 8 + [_I32] * 7 + [_I64] * 14 +
+                                 [_I32, ctypes.c_float, _I32, _P, _SZ, _P, _P], ctypes.c_int),
+    "cast_tree_attn_paged_workspace_size": ([_I32] * 8, _SZ),
     "cast_draft_topk": ([_P, _I64, _I32, _I32, _I32, _I32, _P, _P, _I32, _P, _SZ, _P], ctypes.c_int),
     "cast_draft_topk_workspace_size": ([_I32, _I32, _I32, _I32, _I32], _SZ),
     "cast_build_trees_uniform": ([_P, _P, _I32, _I32, _I32, _I32, _I32] + [_P] * 7, ctypes.c_int),

@@ -57,7 +57,7 @@ constexpr int kCombineUnroll = 8;        // partial loads in flight per thread
 constexpr int kMinChunk = 128;
 constexpr int kQkAhead = 4;   // K and V^T operand reads in flight ahead of their MFMAs
 
-// Where the keys and values of request b, KV head h live.  Two layouts:
+// Where the keys and values of request b, KV head h live.  Three layouts:
 //  concat (store == 0): one ragged [total_kv, Hkv, D] tensor per K and V;
 //      request b owns rows [cu_kv[b], cu_kv[b+1]) = concat(prefix, pack)
 //      (cast_trees/tree_attn.py:71).  pre == pack, pre_b unused.
@@ -66,12 +66,20 @@ constexpr int kQkAhead = 4;   // K and V^T operand reads in flight ahead of thei
 //      at pre + b*pre_b + h*pre_h + t*pre_t; the pack comes from the
 //      forward's own K/V [Hkv, total_q, D], key j at
 //      pack + h*pack_h + (cu_q[b] + j)*pack_t.
+//  pages (store == 1, table set): as store, with prefix key t of request b at
+//      pre + id*kpage + h*pre_h + (t % page_size)*pre_t, id = table[b*table_ld
+//      + t / page_size], pre_b = 0.  page_size is a multiple of 64, so that a
+//      key tile lies within one page, or the table has one page per request.
 struct KvSource {
     const void *k_pre, *v_pre, *k_pack, *v_pack;
     int64_t kpre_b, kpre_h, kpre_t, vpre_b, vpre_h, vpre_t;
     int64_t kpack_h, kpack_t, vpack_h, vpack_t;
     int32_t store, cap;
+    const int32_t *table;
+    int64_t table_ld, kpage, vpage;
+    int32_t page_size;
 };
+enum { kSrcConcat = 0, kSrcStore = 1, kSrcPages = 2 };   // the kernels' instances by layout
 
 // Division of n in [0, 2^31) by a divisor the host knows: (mulhi(m, n) + n) >> s
 // with s = ceil(log2 d) and m = floor(2^32 * (2^s - d) / d) + 1.
@@ -111,7 +119,7 @@ struct AttnArgs {
     float *sk_lse;      // stream-K partial lse [2 * sk_wgs][rows_wg] (partial O at part_o)
     int32_t rows_wg;    // query rows per workgroup (a power of two)
     int32_t rows_shift; // log2(rows_wg)
-    FastDiv by_chunk, by_xcds, by_G;
+    FastDiv by_chunk, by_xcds, by_G, by_page;
     int32_t comb_groups;  // combine kernel: head groups per packed token
     float *part_o;      // [part_rows][Hq][D] fp32, normalised partial outputs
     float *part_lse;    // [part_rows][Hq]    fp32, base-2 partial lse
@@ -513,6 +521,43 @@ struct KvView {
     }
 };
 
+// The pages of one request's prefix, for a workgroup that walks keys from
+// k_begin (a multiple of 64) on: lane j holds the id of the page of keys
+// [64 j, 64 j + 64) behind `from`, loaded 64 tiles ahead, so that a tile's
+// fetch finds its page without a round trip.  The ids of accepted requests
+// were checked (page_check_kernel).
+template <typename T>
+struct PageView {
+    const int32_t *row;
+    const T *k, *v;          // the pool at this KV head
+    int64_t kpage, vpage;
+    int32_t S, page_size, from, ids;
+    FastDiv by_page;
+
+    __device__ __forceinline__ PageView(const AttnArgs &a, const Seq &s, const KvView<T> &kv, int k_begin)
+        : row(a.kv.table + (int64_t)s.b * a.kv.table_ld), k(kv.kpre), v(kv.vpre), kpage(a.kv.kpage), vpage(a.kv.vpage),
+          S(s.S), page_size(a.kv.page_size), by_page(a.by_page) {
+        load(k_begin);
+    }
+    __device__ __forceinline__ void load(int key) {
+        from = key;
+        const int64_t kk = (int64_t)key + (int)(threadIdx.x & 63) * 64;
+        ids = S > 0 ? row[by_page.div((int)min(kk, (int64_t)S - 1))] : 0;
+    }
+    // The page of prefix key t0 (wave-uniform): K and V at its first slot,
+    // that slot, and the prefix keys it holds.
+    struct Page {
+        const T *k, *v;
+        int first, rows;
+    };
+    __device__ __forceinline__ Page at(int t0) {
+        if (t0 - from >= 64 * 64) load(t0 - (t0 - from) % 64);
+        const int64_t id = __builtin_amdgcn_readlane(ids, (t0 - from) >> 6);
+        const int first = by_page.div(t0) * page_size;
+        return {k + id * kpage, v + id * vpage, first, min(page_size, S - first)};
+    }
+};
+
 __device__ __forceinline__ bool pack_bit(int j, uint64_t w0, uint64_t w1) {
     const uint64_t w = j < 64 ? w0 : w1;
     return (w >> (j & 63)) & 1ull;
@@ -522,6 +567,15 @@ __device__ __forceinline__ bool pack_bit(int j, uint64_t w0, uint64_t w1) {
 // MFMA kernel: bf16 or fp16, head_dim D in {64, 128, 256}, WAVES waves x 32
 // query rows.
 // --------------------------------------------------------------------------
+
+// The page view of a workgroup's unit where the instance reads pages.
+template <int SRC, typename T>
+__device__ __forceinline__ auto first_pages(const AttnArgs &a, const Seq &s, int h, int k_begin) {
+    if constexpr (SRC == kSrcPages)
+        return PageView<T>(a, s, KvView<T>(a.kv, s, h), k_begin);
+    else
+        return char{};
+}
 
 // Bits [j0, j0+32) of the 192-bit string {w1 : w0 : 64 ones}, read from bit
 // j0 + 64: pack-relative key positions j < 0 are prefix keys (all visible),
@@ -637,10 +691,11 @@ __device__ __forceinline__ uint32_t nonfinite_rows(const floatx16 (&o)[DB], floa
 // takes head-dim elements 16 i + 8 g + [0, 8) of its key and its query, and
 // the values of keys 8 (e / 4) + 4 g + e % 4, whose weights it holds.  Pack
 // blocks no row sees are skipped as in the kernels.
-template <typename T, typename E, int D>
-__device__ void float_rows(const KvView<T> &kv, int S, int k_begin, int k_end, const T *q, int dr, uint64_t w0,
+template <typename T, typename E, int D, bool PAGES = false>
+__device__ void float_rows(const AttnArgs &a, const Seq &sq, const KvView<T> &kv, int k_begin, int k_end, const T *q, int dr, uint64_t w0,
                            uint64_t w1, float c, floatx16 (&o)[D / 32], float &m, float &l) {
     const int lane = fresh(threadIdx.x & 63), l32 = lane & 31, g = lane >> 5;
+    const int S = sq.S;
 #pragma unroll
     for (int db = 0; db < D / 32; ++db) o[db] = floatx16{};
     m = -INFINITY;
@@ -653,6 +708,12 @@ __device__ void float_rows(const KvView<T> &kv, int S, int k_begin, int k_end, c
         // the block's first row; rows are less than 2^24 bytes apart here
         const T *kb = pack ? kv.kpack + (int64_t)(k0 - S) * kv.kpack_t : kv.kpre + (int64_t)k0 * kv.kpre_t;
         const T *vb = pack ? kv.vpack + (int64_t)(k0 - S) * kv.vpack_t : kv.vpre + (int64_t)k0 * kv.vpre_t;
+        if (PAGES && !pack) {
+            const int at = a.by_page.div(k0), off = k0 - at * a.kv.page_size;
+            const int64_t id = a.kv.table[(int64_t)sq.b * a.kv.table_ld + at];
+            kb = kv.kpre + id * a.kv.kpage + (int64_t)off * kv.kpre_t;
+            vb = kv.vpre + id * a.kv.vpage + (int64_t)off * kv.vpre_t;
+        }
         const int kt = (int)(pack ? kv.kpack_t : kv.kpre_t), vt = (int)(pack ? kv.vpack_t : kv.vpre_t);
         const T *kp = kb + min(l32, n - 1) * kt;   // (keys past the block: masked below)
         floatx16 s = floatx16{};
@@ -967,10 +1028,11 @@ __device__ __forceinline__ bool next_unit(const AttnArgs &a, WorkCursor &cur, Un
 // B = 4, S of 500 to 2000, P of 16 to 64, 32 / 8 heads of 96, fp16: 549 us on
 // the scalar kernel (no split-K, no matrix cores, each key row read by every
 // 16 query rows), 26.4 us here.
-template <int D, int WAVES, bool STORE, typename E, int WPE = 2, bool SKI = false, bool PAD = false>
+template <int D, int WAVES, int SRC, typename E, int WPE = 2, bool SKI = false, bool PAD = false>
 __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WPE)))
 void tree_attn_mfma_kernel(AttnArgs a) {
     using vec8 = typename E::vec8;
+    constexpr bool STORE = SRC != kSrcConcat;
     constexpr int PT = PAD ? E::kTerms : 1;            // 16-bit terms of P
     constexpr float kShift = PAD ? E::kTermShift : 0.f;   // P is scaled by 2^kShift
     constexpr float kSlack = PAD ? E::kTermSlack : kRescaleSlack;
@@ -1068,7 +1130,16 @@ void tree_attn_mfma_kernel(AttnArgs a) {
     // is chosen by a (wave-uniform) branch, not by selecting between the two
     // sources' values, which the compiler may lower to loads through a
     // private array
+    std::conditional_t<SRC == kSrcPages, PageView<uint16_t>, char> pages =
+        first_pages<SRC, uint16_t>(a, wu.sq, wu.h, wu.k_begin);
     auto fetch_tile = [&](const KvView<uint16_t> &v, const Seq &q, int t0) __attribute__((always_inline)) {
+        if constexpr (SRC == kSrcPages) {
+            if (t0 < q.S) {
+                const auto pg = pages.at(t0);
+                fetch_from(pg.k, pg.v, pg.rows, (uint32_t)v.kpre_t * 2u, (uint32_t)v.vpre_t * 2u, (uint32_t)(t0 - pg.first));
+                return;
+            }
+        }
         if (!STORE || t0 < q.S)
             fetch_from(v.kpre, v.vpre, STORE ? q.S : q.T, (uint32_t)v.kpre_t * 2u, (uint32_t)v.vpre_t * 2u,
                        (uint32_t)t0);
@@ -1415,7 +1486,7 @@ void tree_attn_mfma_kernel(AttnArgs a) {
         if (PAD && __builtin_expect(redo != 0, 0)) {
             floatx16 x[DB];
             float mx, sum;
-            float_rows<uint16_t, E, D>(kv, sq.S, k_begin, k_end,
+            float_rows<uint16_t, E, D, SRC == kSrcPages>(a, sq, kv, k_begin, k_end,
                                        qp + (int64_t)fresh(qtok) * a.q_tok + (int64_t)fresh(qhead) * a.q_head, dr, mw0,
                                        mw1, c, x, mx, sum);
             store(x, mx, sum, redo >> l32 & 1);
@@ -1462,9 +1533,10 @@ void tree_attn_mfma_kernel(AttnArgs a) {
 // --------------------------------------------------------------------------
 // PAD: head dims the instances do not name (multiples of 8 below D), the
 // missing elements zeros.
-template <int D, int WAVES, bool STORE, int WPE = 2, bool SKI = false, bool PAD = false>
+template <int D, int WAVES, int SRC, int WPE = 2, bool SKI = false, bool PAD = false>
 __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WPE)))
 void tree_attn_f32_kernel(AttnArgs a) {
+    constexpr bool STORE = SRC != kSrcConcat;
     constexpr uint32_t kNowhere = 0x7ffffff0u;   // byte offset past every source: loads as zeros
     const int dr = PAD ? a.D : D;                // the call's head dim
     constexpr int NT = WAVES * 64;
@@ -1543,8 +1615,16 @@ void tree_attn_f32_kernel(AttnArgs a) {
             }
         }
     };
+    std::conditional_t<SRC == kSrcPages, PageView<float>, char> pages = first_pages<SRC, float>(a, sq, h, k_begin);
     auto fetch = [&](int t) __attribute__((always_inline)) {
         const int t0 = tile_t0(t);
+        if constexpr (SRC == kSrcPages) {
+            if (t < n_pre) {
+                const auto pg = pages.at(t0);
+                fetch_from(pg.k, pg.v, pg.rows, (uint32_t)kv.kpre_t * 4u, (uint32_t)kv.vpre_t * 4u, (uint32_t)(t0 - pg.first));
+                return;
+            }
+        }
         if (!STORE || t < n_pre)
             fetch_from(kv.kpre, kv.vpre, STORE ? sq.S : sq.T, (uint32_t)kv.kpre_t * 4u, (uint32_t)kv.vpre_t * 4u,
                        (uint32_t)t0);
@@ -1809,7 +1889,7 @@ void tree_attn_f32_kernel(AttnArgs a) {
         if (__builtin_expect(redo != 0, 0)) {
             floatx16 x[DB];
             float mx, sum;
-            float_rows<float, Bf16, D>(kv, sq.S, k_begin, k_end,
+            float_rows<float, Bf16, D, SRC == kSrcPages>(a, sq, kv, k_begin, k_end,
                                        qp + (int64_t)fresh(qtok) * a.q_tok + (int64_t)fresh(qhead) * a.q_head, dr, mw0,
                                        mw1, c, x, mx, sum);
             store(x, mx, sum, redo >> l32 & 1);
@@ -2317,53 +2397,59 @@ struct AttnKernel {
     const void *fn;
     int threads;
 };
-template <int DD, int W, int WPE, bool SKI, bool PAD = false>
-static AttnKernel mfma_instance(bool f16, bool store) {
-    const void *fn =
-        f16 ? (store ? reinterpret_cast<const void *>(&tree_attn_mfma_kernel<DD, W, true, Fp16, WPE, SKI, PAD>)
-                     : reinterpret_cast<const void *>(&tree_attn_mfma_kernel<DD, W, false, Fp16, WPE, SKI, PAD>))
-            : (store ? reinterpret_cast<const void *>(&tree_attn_mfma_kernel<DD, W, true, Bf16, WPE, SKI, PAD>)
-                     : reinterpret_cast<const void *>(&tree_attn_mfma_kernel<DD, W, false, Bf16, WPE, SKI, PAD>));
-    return {fn, W * 64};
+// (the layout is one of kSrc*; pages have no stream-K instances)
+template <int DD, int W, int WPE, bool SKI, bool PAD, typename E>
+static const void *mfma_of(int src) {
+    if constexpr (!SKI)
+        if (src == kSrcPages) return reinterpret_cast<const void *>(&tree_attn_mfma_kernel<DD, W, kSrcPages, E, WPE, SKI, PAD>);
+    return src ? reinterpret_cast<const void *>(&tree_attn_mfma_kernel<DD, W, kSrcStore, E, WPE, SKI, PAD>)
+               : reinterpret_cast<const void *>(&tree_attn_mfma_kernel<DD, W, kSrcConcat, E, WPE, SKI, PAD>);
 }
 template <int DD, int W, int WPE, bool SKI, bool PAD = false>
-static AttnKernel f32_instance(bool store) {
-    const void *fn = store ? reinterpret_cast<const void *>(&tree_attn_f32_kernel<DD, W, true, WPE, SKI, PAD>)
-                           : reinterpret_cast<const void *>(&tree_attn_f32_kernel<DD, W, false, WPE, SKI, PAD>);
+static AttnKernel mfma_instance(bool f16, int src) {
+    return {f16 ? mfma_of<DD, W, WPE, SKI, PAD, Fp16>(src) : mfma_of<DD, W, WPE, SKI, PAD, Bf16>(src), W * 64};
+}
+template <int DD, int W, int WPE, bool SKI, bool PAD = false>
+static AttnKernel f32_instance(int src) {
+    if constexpr (!SKI)
+        if (src == kSrcPages)
+            return {reinterpret_cast<const void *>(&tree_attn_f32_kernel<DD, W, kSrcPages, WPE, SKI, PAD>), W * 64};
+    const void *fn = src ? reinterpret_cast<const void *>(&tree_attn_f32_kernel<DD, W, kSrcStore, WPE, SKI, PAD>)
+                         : reinterpret_cast<const void *>(&tree_attn_f32_kernel<DD, W, kSrcConcat, WPE, SKI, PAD>);
     return {fn, W * 64};
 }
 template <bool SKI>
-static AttnKernel attn_kernel_of(int32_t dtype, int32_t D, int waves, bool store) {
+static AttnKernel attn_kernel_of(int32_t dtype, int32_t D, int waves, int src) {
     if (dtype == CAST_FP32) {
-        if (D == 128) return waves == 4 ? f32_instance<128, 4, 2, SKI>(store) : f32_instance<128, 8, 2, SKI>(store);
-        return waves == 4 ? f32_instance<64, 4, 2, SKI>(store) : f32_instance<64, 8, 2, SKI>(store);
+        if (D == 128) return waves == 4 ? f32_instance<128, 4, 2, SKI>(src) : f32_instance<128, 8, 2, SKI>(src);
+        return waves == 4 ? f32_instance<64, 4, 2, SKI>(src) : f32_instance<64, 8, 2, SKI>(src);
     }
     const bool f16 = dtype == CAST_FP16;
     if (D == 128) {
-        return waves == 4 ? mfma_instance<128, 4, 2, SKI>(f16, store) : mfma_instance<128, 8, 2, SKI>(f16, store);
+        return waves == 4 ? mfma_instance<128, 4, 2, SKI>(f16, src) : mfma_instance<128, 8, 2, SKI>(f16, src);
     }
-    return waves == 4 ? mfma_instance<64, 4, 2, SKI>(f16, store) : mfma_instance<64, 8, 2, SKI>(f16, store);
+    return waves == 4 ? mfma_instance<64, 4, 2, SKI>(f16, src) : mfma_instance<64, 8, 2, SKI>(f16, src);
 }
 // Head dims 64 and 128 run 4 or 8 waves; head dim 256 runs 4 (static schedule only).  WPE (waves per
 // SIMD of the register budget) as the kernels' comments give it; sk picks
 // the stream-K instance.
-static AttnKernel attn_kernel(int32_t dtype, int32_t D, int waves, bool store, bool sk) {
+static AttnKernel attn_kernel(int32_t dtype, int32_t D, int waves, int src, bool sk) {
     const bool f16 = dtype == CAST_FP16;
     switch (dtype == CAST_FP32 ? -padded_dim(dtype, D) : padded_dim(dtype, D)) {
-        case 64: return mfma_instance<64, 4, 2, false, true>(f16, store);
-        case 96: return mfma_instance<96, 4, 2, false, true>(f16, store);
-        case 128: return mfma_instance<128, 4, 2, false, true>(f16, store);
-        case 192: return mfma_instance<192, 4, 1, false, true>(f16, store);
-        case 256: return mfma_instance<256, 4, 1, false, true>(f16, store);
-        case -64: return waves == 4 ? f32_instance<64, 4, 2, false, true>(store) : f32_instance<64, 8, 2, false, true>(store);
-        case -128: return waves == 4 ? f32_instance<128, 4, 2, false, true>(store) : f32_instance<128, 8, 2, false, true>(store);
-        case -256: return f32_instance<256, 4, 1, false, true>(store);
+        case 64: return mfma_instance<64, 4, 2, false, true>(f16, src);
+        case 96: return mfma_instance<96, 4, 2, false, true>(f16, src);
+        case 128: return mfma_instance<128, 4, 2, false, true>(f16, src);
+        case 192: return mfma_instance<192, 4, 1, false, true>(f16, src);
+        case 256: return mfma_instance<256, 4, 1, false, true>(f16, src);
+        case -64: return waves == 4 ? f32_instance<64, 4, 2, false, true>(src) : f32_instance<64, 8, 2, false, true>(src);
+        case -128: return waves == 4 ? f32_instance<128, 4, 2, false, true>(src) : f32_instance<128, 8, 2, false, true>(src);
+        case -256: return f32_instance<256, 4, 1, false, true>(src);
         default: break;
     }
     if (D == 256)
-        return dtype == CAST_FP32 ? f32_instance<256, 4, 1, false>(store)
-                                  : mfma_instance<256, 4, 1, false>(f16, store);
-    return sk ? attn_kernel_of<true>(dtype, D, waves, store) : attn_kernel_of<false>(dtype, D, waves, store);
+        return dtype == CAST_FP32 ? f32_instance<256, 4, 1, false>(src)
+                                  : mfma_instance<256, 4, 1, false>(f16, src);
+    return sk ? attn_kernel_of<true>(dtype, D, waves, src) : attn_kernel_of<false>(dtype, D, waves, src);
 }
 
 // Workgroups of kernel k resident on one CU of the current device (1 where
@@ -2558,7 +2644,8 @@ static int tree_attn_run(const void *q, const KvSource &kv, void *out, float *ls
         if (mfma) {
             max_rows = (int32_t)most;
         } else if (limit == CAST_OK && most > 0) {
-            const int64_t longest = kv.store ? (kv.cap > total_q ? kv.cap : total_q) : total_kv;
+            const int64_t rows_of = kv.table ? kv.page_size : kv.cap;
+            const int64_t longest = kv.store ? (rows_of > total_q ? rows_of : total_q) : total_kv;
             if (longest <= most) {
                 mfma = true;
                 max_rows = (int32_t)most;
@@ -2566,6 +2653,12 @@ static int tree_attn_run(const void *q, const KvSource &kv, void *out, float *ls
         }
     }
     if (mfma && limit != CAST_OK) return limit;
+    if (kv.table) {
+        // (a page's rows are addressed as a store's; the scalar kernel reads no pages)
+        if (limit != CAST_OK) return limit;
+        if (!mfma || max_rows < kv.page_size || max_rows < total_q) return CAST_ERR_SHAPE;
+        max_rows = INT32_MAX;
+    }
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     AttnArgs a{};
     a.q = q;
@@ -2596,6 +2689,7 @@ static int tree_attn_run(const void *q, const KvSource &kv, void *out, float *ls
     a.xcds = device_topology().xcds;
     a.by_xcds = fast_div((uint32_t)a.xcds);
     a.by_G = fast_div((uint32_t)a.G);
+    if (kv.table) a.by_page = fast_div((uint32_t)kv.page_size);
 
     if (!mfma) {
         a.chunk = kNoSplit;
@@ -2667,7 +2761,7 @@ static int tree_attn_run(const void *q, const KvSource &kv, void *out, float *ls
     if (a.sk_mode && items < a.sk_wgs) items = a.sk_wgs;
     if (items > 0x7fffffff) return CAST_ERR_SHAPE;
     if (stages & kStageAttn) {
-        const AttnKernel k = attn_kernel(dtype, head_dim, waves, kv.store != 0, a.sk_mode != 0);
+        const AttnKernel k = attn_kernel(dtype, head_dim, waves, kv.table ? kSrcPages : kv.store ? kSrcStore : kSrcConcat, a.sk_mode != 0);
         void *args[] = {&a};
         if (hipLaunchKernel(k.fn, dim3((unsigned)items), dim3(k.threads), args, 0, st) != hipSuccess)
             return CAST_ERR_HIP;
@@ -2773,6 +2867,106 @@ extern "C" int cast_tree_attn_store_fwd(const void *q, const void *k_store, cons
     return tree_attn_run(q, s, out, lse, cu_q, nullptr, prefix_len, pack_len, mask, mask_words, batch, total_q,
                          total_kv, num_q_heads, num_kv_heads, head_dim, q_tok, q_head, o_tok, o_head, dtype,
                          sm_scale, kv_split, workspace, workspace_bytes, status, stream, kStageAttn | kStageCombine);
+}
+
+// --------------------------------------------------------------------------
+// The prefix in pages.  A kernel in front looks every page id of a request
+// over, so that the attention and the combine kernels reject it alike.
+// --------------------------------------------------------------------------
+namespace cast {
+// Request b's prefix length, or -1 where it names a page outside the pool.
+__global__ __launch_bounds__(64) void page_check_kernel(const int32_t *table, int64_t table_ld, int32_t n_pages, int32_t cap,
+                                                        FastDiv by_page, const int32_t *prefix_len, int32_t *checked,
+                                                        int32_t *status) {
+    const int b = blockIdx.x;
+    const int S = prefix_len[b];
+    bool bad = false;
+    if (S > 0 && S <= cap) {
+        const int n = by_page.div(S - 1) + 1;
+        for (int i = threadIdx.x; i < n; i += 64) {
+            const int id = table[(int64_t)b * table_ld + i];
+            bad |= id < 0 || id >= n_pages;
+        }
+    }
+    bad = __any(bad);
+    if (threadIdx.x == 0) {
+        if (bad) raise_flag(status, CAST_FLAG_BAD_PAGE);
+        checked[b] = bad ? -1 : S;
+    }
+}
+}  // namespace cast
+
+// (stream-K has no instances for pages: as for other calls without one, no split)
+static int32_t paged_split(int32_t kv_split) { return kv_split == kSplitStreamK ? -1 : kv_split; }
+
+extern "C" size_t cast_tree_attn_paged_workspace_size(int32_t batch, int32_t total_q, int32_t total_kv,
+                                                      int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                                                      int32_t dtype, int32_t kv_split) {
+    if (batch <= 0) return 0;
+    return align256((size_t)batch * sizeof(int32_t)) +
+           align256(cast_tree_attn_workspace_size(batch, total_q, total_kv, num_q_heads, num_kv_heads, head_dim, dtype,
+                                                  paged_split(kv_split)));
+}
+
+extern "C" int cast_tree_attn_paged_fwd(const void *q, const void *k_pages, const void *v_pages,
+                                        const int32_t *page_table, int64_t table_ld, int32_t max_pages,
+                                        int32_t n_pages, int32_t page_size, const void *k_pack, const void *v_pack,
+                                        void *out, float *lse, const int32_t *cu_q, const int32_t *prefix_len,
+                                        const int32_t *pack_len, const uint64_t *mask, int32_t mask_words,
+                                        int32_t batch, int32_t total_q, int32_t total_kv, int32_t num_q_heads,
+                                        int32_t num_kv_heads, int32_t head_dim, int64_t q_tok, int64_t q_head,
+                                        int64_t kp_page, int64_t kp_head, int64_t kp_tok, int64_t vp_page,
+                                        int64_t vp_head, int64_t vp_tok, int64_t kn_tok, int64_t kn_head,
+                                        int64_t vn_tok, int64_t vn_head, int64_t o_tok, int64_t o_head,
+                                        int32_t dtype, float sm_scale, int32_t kv_split, void *workspace,
+                                        size_t workspace_bytes, int32_t *status, cast_stream_t stream) {
+    if (max_pages < 0 || n_pages < 0 || page_size <= 0 || batch < 0) return CAST_ERR_SHAPE;
+    if (page_size % 64 && max_pages > 1) return CAST_ERR_SHAPE;
+    const int64_t cap = (int64_t)max_pages * page_size;
+    if (cap > INT32_MAX - 4096) return CAST_ERR_SHAPE;
+    if (batch > 0 && total_q > 0 && (!page_table && max_pages)) return CAST_ERR_NULL_POINTER;
+    const int64_t esz = dtype == CAST_FP32 ? 4 : 2;
+    if ((kp_page * esz) % 16 || (vp_page * esz) % 16) return CAST_ERR_ALIGNMENT;
+    KvSource s{};
+    s.k_pre = k_pages;
+    s.v_pre = v_pages;
+    s.k_pack = k_pack;
+    s.v_pack = v_pack;
+    s.kpre_h = kp_head;
+    s.kpre_t = kp_tok;
+    s.vpre_h = vp_head;
+    s.vpre_t = vp_tok;
+    s.kpack_t = kn_tok;
+    s.kpack_h = kn_head;
+    s.vpack_t = vn_tok;
+    s.vpack_h = vn_head;
+    s.store = 1;
+    s.cap = (int32_t)cap;
+    s.table = page_table;
+    s.table_ld = table_ld;
+    s.kpage = kp_page;
+    s.vpage = vp_page;
+    s.page_size = page_size;
+    const size_t head = batch > 0 ? align256((size_t)batch * sizeof(int32_t)) : 0;
+    int32_t *checked = static_cast<int32_t *>(workspace);
+    auto run = [&](int stages) {
+        return tree_attn_run(q, s, out, lse, cu_q, nullptr, stages ? checked : prefix_len, pack_len, mask, mask_words,
+                             batch, total_q, total_kv, num_q_heads, num_kv_heads, head_dim, q_tok, q_head, o_tok, o_head,
+                             dtype, sm_scale, paged_split(kv_split), static_cast<char *>(workspace) + head,
+                             workspace_bytes - head, status, stream, stages);
+    };
+    // the arguments first: no kernel runs on ones the attention refuses
+    if (batch > 0 && total_q > 0) {
+        if (!workspace) return CAST_ERR_NULL_POINTER;
+        if (workspace_bytes < head) return CAST_ERR_WORKSPACE;
+        if (reinterpret_cast<uintptr_t>(workspace) & 255) return CAST_ERR_ALIGNMENT;
+    }
+    const int st = run(0);
+    if (st != CAST_OK || batch == 0 || total_q == 0) return st;
+    page_check_kernel<<<batch, 64, 0, reinterpret_cast<hipStream_t>(stream)>>>(
+        page_table, table_ld, n_pages, s.cap, fast_div((uint32_t)page_size), prefix_len, checked, status);
+    if (hipGetLastError() != hipSuccess) return CAST_ERR_HIP;
+    return run(kStageAttn | kStageCombine);
 }
 
 // --------------------------------------------------------------------------

@@ -1,5 +1,5 @@
-"""A KV cache of pages: append with the rotation on the way, and the attention
-of one new token per request (HIP, gfx950).
+"""A KV cache of pages: append with the rotation on the way, the attention of
+one new token per request, and tree verification over it (HIP, gfx950).
 
   paged_append     rows of new K and V into their requests' pages, K (and Q)
                    rotated to their positions by cos / sin tables; the paged
@@ -7,6 +7,8 @@ of one new token per request (HIP, gfx950).
   paged_attention  one query token per request against the pages: the ordinary
                    decode step (cast_trees/decode.py:211-231 runs it inside the
                    model) beside the tree verification
+  paged_tree_attention  cast_trees/tree_attn.py:116-139 with the prefix read out
+                   of the pages, as store_tree_attention reads it out of a store
 
 A layer's pool is ``[n_pages, Hkv, page_size, D]`` in bfloat16, float16 or
 float32, with any strides of its first three dimensions that keep rows 16-byte
@@ -31,7 +33,7 @@ import operator
 import torch
 
 from . import _lib
-from .tree_attn import _DTYPES, _as_i32, _ready, _require_on
+from .tree_attn import _DTYPES, _as_i32, _host_side, _mask_words, _ready, _require_on, check_host_metadata
 
 
 def _pools(k_pages, v_pages, what):
@@ -259,3 +261,97 @@ def paged_workspace_bytes(batch, max_pages, page_size, H_q, H_kv, D, dtype=torch
     """Bytes of split workspace one ``paged_attention`` call of these sizes needs."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     return _workspace_bytes(dev.index or 0, batch, max_pages, page_size, H_q, H_kv, D, window, _DTYPES[dtype], kv_split)
+
+
+@functools.lru_cache(maxsize=256)
+def _tree_workspace_bytes(device_index, *sizes):
+    """cast_tree_attn_paged_workspace_size of one call's sizes, with the device current."""
+    with _lib.on_device(torch.device("cuda", device_index)):
+        return _lib.load().cast_tree_attn_paged_workspace_size(*sizes)
+
+
+def paged_tree_workspace_bytes(q, k_pages, page_table, total_kv, kv_split=0):
+    """Bytes of workspace one ``paged_tree_attention`` call of these tensors needs."""
+    total_q, H_q, D = q.shape
+    return _tree_workspace_bytes(k_pages.device.index, int(page_table.shape[0]), total_q, int(total_kv), H_q,
+                                 int(k_pages.shape[1]), D, _DTYPES[k_pages.dtype], kv_split)
+
+
+def paged_tree_attention(q, k_pages, v_pages, page_table, k_pack, v_pack, cu_q, prefix_len, pack_len, ancestor_mask,
+                         sm_scale=None, *, total_kv=None, return_lse=False, kv_split=0, check=False, out=None,
+                         workspace=None):
+    """Tree-verification attention whose prefix lies in pages.
+
+    The attention of ``cast_amd.tree_attn.store_tree_attention``, with the same
+    bits over the same tokens: request b's keys are slots [0, prefix_len[b]) of
+    its pages followed by its pack.
+
+      q              [total_q, H_q, D]  (any token/head strides)
+      k_pages/v_pages  pools [n_pages, H_kv, page_size, D], page_size a multiple
+                     of 64 (any size where page_table has one column)
+      k_pack/v_pack  [H_kv, total_q, D] the pass's own K/V
+      total_kv       host bound on sum(prefix_len + pack_len) that sizes launch
+                     and workspace (default B * max_pages * page_size + total_q)
+
+    Returns ``out`` [total_q, H_q, D] (and ``lse`` with ``return_lse``).  A
+    request whose prefix names a page outside the pool is rejected like one with
+    inconsistent lengths: zeros with lse = -inf, and ``check=True`` raises.
+    """
+    lib = _lib.load()
+    kv_split = operator.index(kv_split)
+    n_pages, H_kv, page_size, D = _pools(k_pages, v_pages, "paged_tree_attention")
+    if n_pages == 0:
+        raise ValueError("the pools must hold at least one page")
+    if q.dim() != 3 or q.shape[2] != D:
+        raise ValueError(f"q must be [total_q, H_q, {D}], the pools' head dim")
+    total_q, H_q = int(q.shape[0]), int(q.shape[1])
+    assert H_q % H_kv == 0
+    if tuple(k_pack.shape) != (H_kv, total_q, D) or tuple(v_pack.shape) != (H_kv, total_q, D):
+        raise ValueError(f"k_pack/v_pack must be [{H_kv}, {total_q}, {D}]")
+    if any(t.dtype != k_pages.dtype for t in (q, k_pack, v_pack)):
+        raise ValueError("q, the pools and the pack K/V must share one dtype (the cache is read in place)")
+    dev = k_pages.device
+    _require_on(dev, q=q, v_pages=v_pages, k_pack=k_pack, v_pack=v_pack, out=out, workspace=workspace)
+    esz = q.element_size()
+    q, k_pack, v_pack = _aligned(q, esz), _aligned(k_pack, esz), _aligned(v_pack, esz)
+    page_table = _table(page_table, dev)
+    B, max_pages = (int(x) for x in page_table.shape)
+    if page_size % 64 and max_pages > 1:
+        raise ValueError("paged_tree_attention needs a page size that is a multiple of 64")
+    if total_kv is None:
+        total_kv = B * max_pages * page_size + total_q
+    total_kv = operator.index(total_kv)
+    if not 0 <= total_kv < 1 << 31:
+        raise ValueError("total_kv must be a bound on the summed lengths below 2^31")
+    mask, words = _mask_words(ancestor_mask, total_q, dev)
+    if _host_side(cu_q, prefix_len, pack_len):
+        check_host_metadata(cu_q, prefix_len, pack_len, total_q, total_kv, words, cap=max_pages * page_size)
+    cu_q, prefix_len, pack_len = _as_i32(cu_q, dev), _as_i32(prefix_len, dev), _as_i32(pack_len, dev)
+    if cu_q.shape[0] != B + 1 or prefix_len.shape[0] != B or pack_len.shape[0] != B:
+        raise ValueError("cu_q needs B+1 entries and prefix_len / pack_len B entries (B rows of page_table)")
+    if out is None:
+        out = q.new_empty((total_q, H_q, D))
+    else:
+        if out.shape != q.shape or out.dtype != q.dtype or not _in_place(out, esz):
+            raise ValueError("out must match q's shape and dtype with a contiguous head dim, 16-byte aligned")
+        _no_overlap("out", out)
+    lse = q.new_empty((total_q, H_q), dtype=torch.float32) if return_lse else None
+    if sm_scale is None:
+        sm_scale = 1.0 / math.sqrt(D)
+    dt = _DTYPES[q.dtype]
+    ws_bytes = _tree_workspace_bytes(dev.index, B, total_q, total_kv, H_q, H_kv, D, dt, kv_split)
+    if workspace is None or workspace.numel() * workspace.element_size() < ws_bytes:
+        workspace = q.new_empty(ws_bytes, dtype=torch.uint8)
+    status = torch.zeros(1, dtype=torch.int32, device=dev) if check else None
+    with _lib.on_device(dev):
+        st = lib.cast_tree_attn_paged_fwd(
+            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), page_table.stride(0), max_pages,
+            n_pages, page_size, k_pack.data_ptr(), v_pack.data_ptr(), out.data_ptr(), _lib.ptr(lse), cu_q.data_ptr(),
+            prefix_len.data_ptr(), pack_len.data_ptr(), mask.data_ptr(), words, B, total_q, total_kv, H_q, H_kv, D,
+            *q.stride()[:2], *k_pages.stride()[:3], *v_pages.stride()[:3], *k_pack.stride()[1::-1],
+            *v_pack.stride()[1::-1], *out.stride()[:2], dt, float(sm_scale), kv_split, workspace.data_ptr(), ws_bytes,
+            _lib.ptr(status), _lib.stream_of(q))
+    _lib.check(st, "cast_tree_attn_paged_fwd")
+    if check:
+        _lib.raise_device_flags(status.item(), "paged_tree_attention")
+    return (out, lse) if return_lse else out

@@ -458,6 +458,38 @@ size_t cast_paged_attn_workspace_size(int32_t batch, int32_t max_pages, int32_t 
                                       int32_t head_dim, int32_t window, int32_t dtype,
                                       int32_t kv_split);
 
+/* ---------------------------------------------------------------------
+ * K2 with the prefix in pages: cast_tree_attn_store_fwd where request b's
+ * prefix_len[b] stored tokens lie in its pages; the pack's K and V are the
+ * forward's own (kn_*, vn_*: token and head strides).  Same kernels, same
+ * results as over a store that holds the same tokens.
+ *   page_size  a multiple of 64, or any size where max_pages is 1; n_pages
+ *            bounds the ids (a request whose prefix names another page is
+ *            rejected: CAST_FLAG_BAD_PAGE and _BAD_OFFSETS)
+ *   total_kv a bound on sum_b (prefix_len[b] + pack_len[b])
+ *   workspace  cast_tree_attn_paged_workspace_size(...) bytes, 256-byte
+ *            aligned, always needed (the checked lengths lie in it)
+ *   kv_split CAST_SPLIT_STREAM runs unsplit
+ * A kernel in front checks the page ids.  Head dims and alignment that take
+ * the scalar kernel elsewhere are refused here.
+ * ------------------------------------------------------------------- */
+int cast_tree_attn_paged_fwd(const void *q, const void *k_pages, const void *v_pages,
+                             const int32_t *page_table, int64_t table_ld, int32_t max_pages,
+                             int32_t n_pages, int32_t page_size, const void *k_pack,
+                             const void *v_pack, void *out, float *lse, const int32_t *cu_q,
+                             const int32_t *prefix_len, const int32_t *pack_len,
+                             const uint64_t *mask, int32_t mask_words, int32_t batch,
+                             int32_t total_q, int32_t total_kv, int32_t num_q_heads,
+                             int32_t num_kv_heads, int32_t head_dim, int64_t q_tok, int64_t q_head,
+                             int64_t kp_page, int64_t kp_head, int64_t kp_tok, int64_t vp_page,
+                             int64_t vp_head, int64_t vp_tok, int64_t kn_tok, int64_t kn_head,
+                             int64_t vn_tok, int64_t vn_head, int64_t o_tok, int64_t o_head,
+                             int32_t dtype, float sm_scale, int32_t kv_split, void *workspace,
+                             size_t workspace_bytes, int32_t *status, cast_stream_t stream);
+size_t cast_tree_attn_paged_workspace_size(int32_t batch, int32_t total_q, int32_t total_kv,
+                                           int32_t num_q_heads, int32_t num_kv_heads,
+                                           int32_t head_dim, int32_t dtype, int32_t kv_split);
+
 
 #ifdef __cplusplus
 }

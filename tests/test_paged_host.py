@@ -119,3 +119,40 @@ def test_python_refusals():
     for flag in (_lib.FLAG_BAD_PAGE, _lib.FLAG_BAD_POSITION):
         with pytest.raises(ValueError):
             _lib.raise_device_flags(flag, "x")
+
+
+def tree(lib, **over):
+    a = dict(ptrs=[FAKE] * 3, table=FAKE, ld=4, max_pages=4, n_pages=8, ps=64, more=[FAKE] * 8, words=2, B=1, tq=16, tkv=64,
+             Hq=8, Hkv=2, D=128, s=[128] * 14, dtype=0, scale=0.1, split=-1, ws=FAKE, wsb=1 << 20, status=None, stream=None)
+    a.update(over)
+    return lib.cast_tree_attn_paged_fwd(*a["ptrs"], a["table"], a["ld"], a["max_pages"], a["n_pages"], a["ps"],
+                                        *a["more"], a["words"], a["B"], a["tq"], a["tkv"], a["Hq"], a["Hkv"], a["D"],
+                                        *a["s"], a["dtype"], a["scale"], a["split"], a["ws"], a["wsb"], a["status"],
+                                        a["stream"])
+
+
+def test_tree_host_validation(lib):
+    assert tree(lib, B=0) == 0 and tree(lib, tq=0) == 0
+    assert tree(lib, ps=0) == 7 and tree(lib, ps=48) == 7 and tree(lib, max_pages=-1) == 7
+    assert tree(lib, max_pages=1 << 20, ps=1 << 12) == 7
+    assert tree(lib, Hkv=3) == 2 and tree(lib, dtype=2) == 4 and tree(lib, scale=0.0) == 9 and tree(lib, words=3) == 7
+    assert tree(lib, table=None) == 1 and tree(lib, ptrs=[None] * 3) == 1 and tree(lib, more=[None] * 8) == 1
+    assert tree(lib, ws=None) == 1 and tree(lib, wsb=255) == 8 and tree(lib, ws=FAKE + 16) == 6
+    assert tree(lib, D=12) == 5
+    assert tree(lib, s=[128, 128, 4] + [128] * 11) == 6                 # page stride
+    # what the scalar kernel takes elsewhere is refused: unaligned strides, rows too far apart
+    assert tree(lib, D=96, s=[4] + [128] * 13) == 6
+    assert tree(lib, D=96, s=[128] * 4 + [1 << 24] + [128] * 9) == 7
+    need = lib.cast_tree_attn_paged_workspace_size(8, 1024, 66560, 32, 8, 128, 0, 64)
+    assert need > lib.cast_tree_attn_workspace_size(8, 1024, 66560, 32, 8, 128, 0, 64)
+    assert tree(lib, B=8, tq=1024, tkv=66560, Hq=32, Hkv=8, split=64, wsb=need - 1) == 8
+    # stream-K has no instances here: sized as unsplit
+    assert lib.cast_tree_attn_paged_workspace_size(8, 1024, 66560, 32, 8, 128, 0, -2) == 256
+
+
+def test_tree_python_refusals():
+    from cast_amd import paged_tree_attention
+    pool, q = torch.zeros((2, 2, 64, 64)), torch.zeros((4, 4, 64))
+    with pytest.raises(ValueError, match="on the GPU"):
+        paged_tree_attention(q, pool, pool, torch.zeros((1, 1), dtype=torch.int32), torch.zeros((2, 4, 64)),
+                             torch.zeros((2, 4, 64)), [0, 4], [0], [4], torch.zeros(4, dtype=torch.int64))
