@@ -12,6 +12,10 @@ Mirrors the attention side of cast_trees/serving.py:
   begin_verify        the packing half of BatchedServer._verify_varlen
                       (serving.py:208-253): packed tokens, positions,
                       offsets and ancestor words, then PLAN.set
+  begin_decode        an ordinary step of one new token per request over the
+                      same store (what cast_trees/decode.py:211-231 does for
+                      one request): the hook appends each layer's K/V and
+                      attends with cast_amd.paged_attention
   append_store        BatchedServer._append_store (serving.py:264-289): the
                       accepted rows of every layer into the store in one
                       launch; append_accepted does it from greedy_accept's
@@ -30,6 +34,11 @@ store's dtype (bf16 products are exact in the fp32 MFMA accumulators, so the
 up-cast adds no precision to the score dot products; the probabilities are
 rounded to bf16 before the value product, as the reference kernel does for
 bf16 inputs, tree_attn.py:66,87).
+
+Stores may also be pools of pages [n_pages, Hkv, page_size, D] with a
+``page_table`` int32 [B, max_pages] (see cast_amd.paged): begin_verify,
+begin_decode and append_accepted take it, and the hook then reads and writes
+the pages in place.
 """
 from __future__ import annotations
 
@@ -40,6 +49,7 @@ import numpy as np
 import torch
 import torch.nn.functional as F
 
+from .paged import paged_append, paged_attention, paged_tree_attention, paged_tree_workspace_bytes
 from .tree import MAX_PACK
 from .tree_attn import store_tree_attention
 from .verify import _i32_on, tree_bitmask
@@ -56,8 +66,11 @@ class VerifyPassState:
         self.active = False
         self.layer = 0
         self.workspace = None
+        self.page_table = None
+        self.decode = False
 
     def set(self, **fields):
+        self.page_table, self.decode = None, False
         for name, value in fields.items():
             setattr(self, name, value)
         self.layer = 0
@@ -68,6 +81,8 @@ class VerifyPassState:
         self.buf_k = None
         self.buf_v = None
         self.workspace = None
+        self.page_table = None
+        self.decode = False
 
 
 PLAN = VerifyPassState()
@@ -146,6 +161,8 @@ def _varlen_attention(module, query, key, value, attention_mask, scaling=None, d
     if not PLAN.active:
         return _plain_attention(query, key, value, attention_mask, scaling)
 
+    if PLAN.decode:
+        return _decode_attention(query, key, value, scaling, kw)
     li = PLAN.layer
     PLAN.layer += 1
     while len(PACK_KV["k"]) <= li:
@@ -161,6 +178,14 @@ def _varlen_attention(module, query, key, value, attention_mask, scaling=None, d
         q = q.to(dt)
     if k_pack.dtype != dt:
         k_pack, v_pack = k_pack.to(dt), v_pack.to(dt)
+    if PLAN.page_table is not None:
+        if PLAN.workspace is None:
+            PLAN.workspace = torch.empty(paged_tree_workspace_bytes(q, buf_k, PLAN.page_table, PLAN.total_kv),
+                                         dtype=torch.uint8, device=q.device)
+        out = paged_tree_attention(q, buf_k, buf_v, PLAN.page_table, k_pack, v_pack, PLAN.cu_q, PLAN.prefix_len,
+                                   PLAN.pack_len, PLAN.ancestor_mask, sm_scale=scaling, total_kv=PLAN.total_kv,
+                                   workspace=PLAN.workspace)
+        return out.to(query.dtype).unsqueeze(0), None
     if getattr(PLAN, "workspace", None) is None:
         # split-K scratch, sized once per pass and shared by every layer
         PLAN.workspace = torch.empty(max(workspace_bytes(q, buf_k, PLAN.total_kv), 256), dtype=torch.uint8,
@@ -168,6 +193,24 @@ def _varlen_attention(module, query, key, value, attention_mask, scaling=None, d
     out = store_tree_attention(q, buf_k, buf_v, k_pack, v_pack, PLAN.cu_q, PLAN.prefix_len, PLAN.pack_len,
                                PLAN.ancestor_mask, sm_scale=scaling, total_kv=PLAN.total_kv,
                                workspace=PLAN.workspace)
+    return out.to(query.dtype).unsqueeze(0), None
+
+
+def _decode_attention(query, key, value, scaling, kw):
+    """The hook's part of an ordinary decode step (begin_decode): query [1, Hq,
+    B, D] and key/value [1, Hkv, B, D] hold one token per request.  Its K and V
+    go behind the request's stored tokens, then it attends to all of them.  The
+    forward's own ``softcap`` and ``sliding_window`` are honoured."""
+    li = PLAN.layer
+    PLAN.layer += 1
+    buf_k, buf_v = PLAN.buf_k[li], PLAN.buf_v[li]
+    dt = buf_k.dtype
+    q, k, v = (x.select(0, 0).transpose(0, 1) for x in (query, key, value))   # [B, H, D] views
+    if k.dtype != dt:
+        k, v = k.to(dt), v.to(dt)
+    paged_append(k, v, buf_k, buf_v, PLAN.page_table, PLAN.prefix_len, new_len=PLAN.new_len)
+    out = paged_attention(q if q.dtype == dt else q.to(dt), buf_k, buf_v, PLAN.page_table, PLAN.new_len, scaling,
+                          softcap=kw.get("softcap") or 0.0, window=kw.get("sliding_window") or 0)
     return out.to(query.dtype).unsqueeze(0), None
 
 
@@ -181,10 +224,54 @@ def workspace_bytes(q, buf_k, total_kv):
                                                          _DTYPES[buf_k.dtype], 0))
 
 
-def begin_verify(buf_k, buf_v, store_len, roots, trees, seq_lens, device=None):
+def _page_rows(page_table, batch, dev):
+    """page_table as the int32 [batch, max_pages] device tensor the kernels read."""
+    t = torch.as_tensor(page_table)
+    if t.dim() != 2 or t.shape[0] != batch:
+        raise ValueError(f"page_table must be [{batch}, max_pages], a row per request")
+    return _i32_on(t, dev)
+
+
+def begin_decode(buf_k, buf_v, store_len, tokens, page_table=None, device=None):
+    """Arm the hook for one ordinary decode step of B requests, a token each.
+
+    buf_k / buf_v: per-layer stores [B, Hkv, cap, D], or pools of pages with
+    ``page_table`` [B, max_pages]; store_len[b]: tokens of request b in the
+    store; tokens[b]: its new token, at position store_len[b].  Returns
+    (input_ids [1, B], position_ids [1, B], new_len): the forward runs with
+    ``_attn_implementation = "cast_varlen"``, every layer appends its K/V and
+    attends, and new_len (int32 [B] on the device) holds the lengths after it;
+    call ``PLAN.clear()`` afterwards.  store_len may be a device tensor (the
+    step before's new_len): nothing then copies to or from the host.
+    """
+    dev = torch.device(device) if device is not None else buf_k[0].device
+    n = int(buf_k[0].shape[0])
+    on_host = not (isinstance(store_len, torch.Tensor) and store_len.is_cuda)
+    B = len(store_len)
+    if page_table is None:
+        if B != n:
+            raise ValueError("store_len needs one entry per request of the store")
+        cap = int(buf_k[0].shape[2])
+        table = torch.arange(n, dtype=torch.int32, device=dev)[:, None]
+    else:
+        table = _page_rows(page_table, B, dev)
+        cap = int(table.shape[1]) * int(buf_k[0].shape[2])
+    if on_host and B and not 0 <= min(int(x) for x in store_len) <= max(int(x) for x in store_len) < cap:
+        raise ValueError("store_len leaves no room for the new token")
+    lens = _i32_on(store_len, dev)
+    ids = torch.as_tensor(tokens, device=dev).to(torch.long).view(1, -1)
+    if ids.shape[1] != B:
+        raise ValueError("tokens needs one entry per request")
+    PLAN.set(buf_k=buf_k, buf_v=buf_v, prefix_len=lens, new_len=torch.empty_like(lens), page_table=table, decode=True,
+             workspace=None)
+    return ids, lens.to(torch.long).view(1, -1), PLAN.new_len
+
+
+def begin_verify(buf_k, buf_v, store_len, roots, trees, seq_lens, device=None, page_table=None):
     """Pack B trees for one verify forward and activate the hook.
 
-    buf_k / buf_v: per-layer stores [B, Hkv, cap, D]; store_len[b]: tokens of
+    buf_k / buf_v: per-layer stores [B, Hkv, cap, D], or pools of pages with
+    ``page_table`` [B, max_pages]; store_len[b]: tokens of
     request b in the store; roots[b]: the root token (last committed token);
     trees[b]: its TreeNode list; seq_lens[b]: the root's position.  Returns
     (input_ids [1, total_q], position_ids [1, total_q], cu_q list), the inputs
@@ -197,6 +284,9 @@ def begin_verify(buf_k, buf_v, store_len, roots, trees, seq_lens, device=None):
     if max(pack_len) > MAX_PACK:
         raise ValueError(f"a pack holds at most {MAX_PACK} tokens (root + {MAX_PACK - 1} nodes)")
     cap = int(buf_k[0].shape[2])
+    if page_table is not None:
+        page_table = _page_rows(page_table, B, dev)
+        cap *= int(page_table.shape[1])
     if max(store_len) > cap:
         raise ValueError("store_len exceeds the store capacity")
     tok, pos, parent = [], [], []
@@ -223,7 +313,8 @@ def begin_verify(buf_k, buf_v, store_len, roots, trees, seq_lens, device=None):
     PACK_KV["k"], PACK_KV["v"] = [None] * n_layers, [None] * n_layers
     _PACK_REC.begin(n_layers)
     PLAN.set(buf_k=buf_k, buf_v=buf_v, prefix_len=prefix_t, pack_len=pack_t, cu_q=cu_q_t,
-             total_kv=int(sum(store_len)) + total_q, ancestor_mask=words, parent=parent_t, workspace=None)
+             total_kv=int(sum(store_len)) + total_q, ancestor_mask=words, parent=parent_t, workspace=None,
+             page_table=page_table, decode=False)
     ids = torch.tensor([tok], dtype=torch.long, device=dev)
     pos_ids = torch.tensor([pos], dtype=torch.long, device=dev)
     return ids, pos_ids, cu_q
@@ -330,9 +421,34 @@ def _append_launch(buf_k, buf_v, pack_k, pack_v, src_row, path, path_len, store_
     _lib.check(st, "cast_store_append")
 
 
-def append_accepted(buf_k, buf_v, store_len, cu_q, path, path_len, pack_k=None, pack_v=None, *, check=False):
+def _append_pages(buf_k, buf_v, pack_k, pack_v, page_table, cu_q, path, path_len, store_len, new_len, status):
+    """The accepted rows of every layer into the layers' pools of pages, one
+    launch per 64 layers.  Stream-ordered, no host sync."""
+    from . import _lib
+    from .tree_attn import _DTYPES
+    lay = _store_layout(buf_k, buf_v)
+    dev = lay["device"]
+    rec = _PACK_REC.arrays_for(lay, pack_k, pack_v)
+    kp, vp, kp_st, vp_st, total_q = rec if rec is not None else _pack_arrays(lay, pack_k, pack_v)
+    n = int(store_len.shape[0])
+    table = _page_rows(page_table, n, dev)
+    if cu_q.shape[0] != n + 1 or path_len.shape[0] < n or path.dim() != 2 or path.shape[0] < n or path.shape[1] < MAX_PACK:
+        raise ValueError("cu_q must be [B + 1], path_len [B] and path [B, >=128], as written by greedy_accept")
+    with _lib.on_device(dev):
+        st = _lib.load().cast_paged_append(
+            kp, vp, lay["k"], lay["v"], lay["L"], _lib.ptr(table), table.stride(0), int(table.shape[1]), lay["B"],
+            lay["cap"], _lib.ptr(store_len), _lib.ptr(new_len), n, total_q, _lib.ptr(cu_q), _lib.ptr(path),
+            path.stride(0), _lib.ptr(path_len), None, None, None, None, None, 0, 0, 0, 0, None, 0, lay["Hkv"], lay["D"],
+            *kp_st, *vp_st, *lay["store_k"], *lay["store_v"], 0, 0, 0, 0, 0, 0, _DTYPES[lay["dtype"]],
+            _lib.ptr(status), _lib.stream_of(buf_k[0]))
+    _lib.check(st, "cast_paged_append")
+
+
+def append_accepted(buf_k, buf_v, store_len, cu_q, path, path_len, pack_k=None, pack_v=None, *, page_table=None,
+                    check=False):
     """Append every request's root and accepted nodes to its store slot, all
     layers in one launch, straight from greedy_accept's device outputs.
+    With ``page_table`` the stores are pools of pages.
 
     store_len, cu_q: int32 device tensors [B] / [B+1]; path int32 [B, 128],
     path_len int32 [B] (greedy_accept).  pack_k / pack_v default to PACK_KV.
@@ -345,8 +461,13 @@ def append_accepted(buf_k, buf_v, store_len, cu_q, path, path_len, pack_k=None, 
     cu_q = _i32_on(cu_q, dev)
     new_len = torch.empty_like(store_len)
     status = torch.zeros(1, dtype=torch.int32, device=dev) if check else None
-    _append_launch(buf_k, buf_v, pack_k, pack_v, cu_q[:-1], _i32_on(path, dev), _i32_on(path_len, dev), store_len,
-                   new_len, status)
+    path, path_len = _i32_on(path, dev), _i32_on(path_len, dev)
+    if page_table is not None:
+        if dev.type != "cuda":
+            raise ValueError("the KV append runs on the GPU: stores and packs must be device tensors")
+        _append_pages(buf_k, buf_v, pack_k, pack_v, page_table, cu_q, path, path_len, store_len, new_len, status)
+    else:
+        _append_launch(buf_k, buf_v, pack_k, pack_v, cu_q[:-1], path, path_len, store_len, new_len, status)
     if check:
         from . import _lib
         _lib.raise_device_flags(status.item(), "append_accepted")
