@@ -26,8 +26,6 @@ constexpr int kPagedThreads = 256;
 constexpr int kPathRows = 8;                // workgroups that share a request's accepted rows
 
 struct PagedAppendArgs {
-    const void *k[kPagedLayersPerLaunch], *v[kPagedLayersPerLaunch];
-    void *k_pages[kPagedLayersPerLaunch], *v_pages[kPagedLayersPerLaunch];
     const void *q;
     void *q_out, *k_out;
     const float *cos, *sin;
@@ -44,6 +42,14 @@ struct PagedAppendArgs {
     int32_t units;          // threads per rotated head: a pair of chunks each in the half style
     int32_t tasks;          // threads per token
     int32_t rows;           // workgroups (x) that move rows; the ones behind check one request each
+};
+
+// The layers' addresses of one launch, of 1 or kPagedLayersPerLaunch layers:
+// a launch copies its arguments, and 2 KiB of them show in a small call.
+template <int LAYERS>
+struct PagedLayers {
+    const void *k[LAYERS], *v[LAYERS];
+    void *k_pages[LAYERS], *v_pages[LAYERS];
 };
 
 // Row j of request b: source row, slot, page and offset, and the rotation's
@@ -91,17 +97,23 @@ __device__ __forceinline__ bool paged_request(const PagedAppendArgs &a, int b, i
     return root >= 0 && n >= 0 && (int64_t)root + n <= a.total;
 }
 
-// The request of packed row `row`: as many as end at or before it.  Wave-wide
-// loads of 64 ends at a time.
-__device__ __forceinline__ int request_of(const PagedAppendArgs &a, int row) {
+// The request of packed row `row` - as many as end at or before it - with its
+// first row, end and length in the cache: one round of loads per 64 requests.
+__device__ __forceinline__ int request_of(const PagedAppendArgs &a, int row, int &root, int &end, int &S) {
     const int lane = threadIdx.x & 63;
-    int b = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
-        const uint64_t past = __ballot(b0 + lane < a.batch && a.cu_q[b0 + lane + 1] <= row);
-        b += __popcll(past);
-        if (~past) break;
+        const int b = min(b0 + lane, a.batch - 1);
+        const int c0 = a.cu_q[b], c1 = a.cu_q[b + 1], len = a.seq_len[b];
+        const uint64_t past = __ballot(c1 <= row);
+        if (~past) {
+            const int at = __builtin_ctzll(~past);
+            root = __builtin_amdgcn_readlane(c0, at);
+            end = __builtin_amdgcn_readlane(c1, at);
+            S = __builtin_amdgcn_readlane(len, at);
+            return b0 + at;
+        }
     }
-    return __builtin_amdgcn_readfirstlane(b);
+    return a.batch;
 }
 
 // One chunk's elements as floats, and back.
@@ -150,10 +162,10 @@ __device__ __forceinline__ void load_angles(const float *p, float (&x)[8]) {
     }
 }
 
-template <typename E>
-__global__ __launch_bounds__(kPagedThreads) void paged_append_kernel(PagedAppendArgs a) {
+template <typename E, int LAYERS>
+__global__ __launch_bounds__(kPagedThreads) void paged_append_kernel(PagedAppendArgs a, PagedLayers<LAYERS> at) {
     constexpr int EPC = __is_same(E, Fp32) ? 4 : 8;   // elements per 16-byte chunk
-    const int layer = blockIdx.z;
+    const int layer = LAYERS == 1 ? 0 : blockIdx.z;
     if ((int)blockIdx.x >= a.rows) {
         // ---- one request's check, by its own workgroup: any row that cannot
         // be placed leaves its length as it was
@@ -192,45 +204,29 @@ __global__ __launch_bounds__(kPagedThreads) void paged_append_kernel(PagedAppend
     const bool paired = kind < 2 && !a.interleaved && unit < half;
     const int chunk = kind < 2 && !a.interleaved && !paired ? unit + half : unit;
 
-    int b, j0, step, root, n;
-    if (a.path) {
-        b = blockIdx.x / kPathRows;
-        j0 = blockIdx.x % kPathRows;
-        step = kPathRows;
-    } else {
-        b = a.cu_q ? request_of(a, blockIdx.x) : (int)blockIdx.x;
-        if (b >= a.batch) return;   // rows behind the last request
-        j0 = 0;
-        step = 1;
-    }
-    if (!paged_request(a, b, root, n)) return;
-    if (!a.path) {
-        j0 = blockIdx.x - root;
-        if (j0 < 0 || j0 >= n) return;
-        n = j0 + 1;
-    }
-    const int S = a.seq_len[b];
-    for (int j = j0; j < n; j += step) {
-        const PagedRow r = paged_row(a, b, root, j, S);
-        if (r.flags || !live) continue;
-        const int64_t src = r.src;
-        const char *from;
+    const int64_t far = half * 16;   // from a pair's first chunk to its second
+    const char *rows = static_cast<const char *>(kind == 0 ? a.q : kind == 1 ? at.k[layer] : at.v[layer]);
+    const int64_t row_step = kind == 0 ? a.q_tok : kind == 1 ? a.k_tok : a.v_tok;
+    rows += head * (kind == 0 ? a.q_head : kind == 1 ? a.k_head : a.v_head) + chunk * 16;
+    u32x4 x{}, y{};
+    auto load = [&](int64_t src) __attribute__((always_inline)) {
+        if (!live) return;
+        x = *reinterpret_cast<const u32x4 *>(rows + src * row_step);
+        if (paired) y = *reinterpret_cast<const u32x4 *>(rows + src * row_step + far);
+    };
+    auto put = [&](const PagedRow &r) __attribute__((always_inline)) {
         char *to, *also = nullptr;   // also: k_out
+        const int64_t src = r.src;
         if (kind == 0) {
-            from = static_cast<const char *>(a.q) + src * a.q_tok + head * a.q_head;
             to = static_cast<char *>(a.q_out) + src * a.qo_tok + head * a.qo_head;
         } else if (kind == 1) {
-            from = static_cast<const char *>(a.k[layer]) + src * a.k_tok + head * a.k_head;
-            to = static_cast<char *>(a.k_pages[layer]) + r.page * a.kp_page + head * a.kp_head + r.offset * a.kp_tok;
-            if (a.k_out) also = static_cast<char *>(a.k_out) + src * a.ko_tok + head * a.ko_head;
+            to = static_cast<char *>(at.k_pages[layer]) + r.page * a.kp_page + head * a.kp_head + r.offset * a.kp_tok;
+            if (a.k_out) also = static_cast<char *>(a.k_out) + src * a.ko_tok + head * a.ko_head + chunk * 16;
         } else {
-            from = static_cast<const char *>(a.v[layer]) + src * a.v_tok + head * a.v_head;
-            to = static_cast<char *>(a.v_pages[layer]) + r.page * a.vp_page + head * a.vp_head + r.offset * a.vp_tok;
+            to = static_cast<char *>(at.v_pages[layer]) + r.page * a.vp_page + head * a.vp_head + r.offset * a.vp_tok;
         }
-        u32x4 x = *reinterpret_cast<const u32x4 *>(from + chunk * 16);
+        to += chunk * 16;
         if (paired) {
-            const int far = (chunk + half) * 16;
-            u32x4 y = *reinterpret_cast<const u32x4 *>(from + far);
             float xf[8], yf[8], c[8], s[8], xr[8], yr[8];
             load_angles<EPC>(a.cos + r.pos * a.rope_ld + chunk * EPC, c);
             load_angles<EPC>(a.sin + r.pos * a.rope_ld + chunk * EPC, s);
@@ -257,9 +253,53 @@ __global__ __launch_bounds__(kPagedThreads) void paged_append_kernel(PagedAppend
             }
             x = round_chunk<E>(xr);
         }
-        *reinterpret_cast<u32x4 *>(to + chunk * 16) = x;
-        if (also) *reinterpret_cast<u32x4 *>(also + chunk * 16) = x;
+        *reinterpret_cast<u32x4 *>(to) = x;
+        if (also) *reinterpret_cast<u32x4 *>(also) = x;
+    };
+
+    if (a.path) {
+        const int b = blockIdx.x / kPathRows;
+        int root, n;
+        if (!paged_request(a, b, root, n)) return;
+        const int S = a.seq_len[b];
+        for (int j = blockIdx.x % kPathRows; j < n; j += kPathRows) {
+            const PagedRow r = paged_row(a, b, root, j, S);
+            if (r.flags || !live) continue;
+            load(r.src);
+            put(r);
+        }
+        return;
     }
+    // the row is known: its loads run beside the lookups of where it goes
+    const int row = blockIdx.x;
+    load(row);
+    int b = row, root = row, end = row + 1, S;
+    if (a.cu_q) {
+        b = request_of(a, row, root, end, S);
+        // rows behind the last request, offsets that make no sense
+        if (b >= a.batch || root < 0 || root > row || end > a.total) return;
+    } else {
+        S = a.seq_len[b];
+    }
+    const PagedRow r = paged_row(a, b, root, row - root, S);
+    if (r.flags || !live) return;
+    put(r);
+}
+
+template <int LAYERS>
+static int launch_append(const PagedAppendArgs &a, const void *const *k, const void *const *v, void *const *k_pages,
+                         void *const *v_pages, int32_t n, int32_t dtype, dim3 grid, hipStream_t st) {
+    PagedLayers<LAYERS> at{};
+    for (int32_t l = 0; l < n; ++l) {
+        at.k[l] = k[l];
+        at.v[l] = v[l];
+        at.k_pages[l] = k_pages[l];
+        at.v_pages[l] = v_pages[l];
+    }
+    if (dtype == CAST_BF16) paged_append_kernel<Bf16, LAYERS><<<grid, kPagedThreads, 0, st>>>(a, at);
+    else if (dtype == CAST_FP16) paged_append_kernel<Fp16, LAYERS><<<grid, kPagedThreads, 0, st>>>(a, at);
+    else paged_append_kernel<Fp32, LAYERS><<<grid, kPagedThreads, 0, st>>>(a, at);
+    return hipGetLastError() == hipSuccess ? CAST_OK : CAST_ERR_HIP;
 }
 
 }  // namespace cast
@@ -362,21 +402,15 @@ extern "C" int cast_paged_append(const void *const *k, const void *const *v, voi
     a.rows = (int32_t)rows;
     for (int32_t l0 = 0; l0 < layers; l0 += kPagedLayersPerLaunch) {
         const int32_t n = layers - l0 < kPagedLayersPerLaunch ? layers - l0 : kPagedLayersPerLaunch;
-        for (int32_t l = 0; l < n; ++l) {
-            a.k[l] = k[l0 + l];
-            a.v[l] = v[l0 + l];
-            a.k_pages[l] = k_pages[l0 + l];
-            a.v_pages[l] = v_pages[l0 + l];
-        }
         const bool checks = l0 == 0 && (new_len || status);
         a.new_len = checks ? new_len : nullptr;
         const dim3 grid((unsigned)(a.rows + (checks ? batch : 0)), (unsigned)slices, (unsigned)n);
         if (grid.x == 0) continue;
         hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-        if (dtype == CAST_BF16) paged_append_kernel<Bf16><<<grid, kPagedThreads, 0, st>>>(a);
-        else if (dtype == CAST_FP16) paged_append_kernel<Fp16><<<grid, kPagedThreads, 0, st>>>(a);
-        else paged_append_kernel<Fp32><<<grid, kPagedThreads, 0, st>>>(a);
-        if (hipGetLastError() != hipSuccess) return CAST_ERR_HIP;
+        const int rc = n == 1 ? launch_append<1>(a, k + l0, v + l0, k_pages + l0, v_pages + l0, 1, dtype, grid, st)
+                              : launch_append<kPagedLayersPerLaunch>(a, k + l0, v + l0, k_pages + l0, v_pages + l0, n, dtype,
+                                                                     grid, st);
+        if (rc != CAST_OK) return rc;
     }
     return CAST_OK;
 }

@@ -532,71 +532,92 @@ __global__ __launch_bounds__(kPWaves * 64) void paged_attn_kernel(PagedAttnArgs 
     }
 }
 
-// Joins the splits of one (request, query head) per wave.
-template <typename E>
+// Joins the splits of one (request, query head): groups of LP lanes, one
+// float4 of the head dim a lane, walk every NG-th split with up to four in
+// flight and their own running maximum, then join through LDS.
+template <typename E, int LP>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
     using T = typename E::T;
-    const int b = blockIdx.y, lane = threadIdx.x & 63;
-    const int head = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (head >= a.Hq) return;
+    constexpr int NG = 256 / LP;
+    __shared__ __attribute__((aligned(16))) floatx4 Os[NG][LP];
+    __shared__ float ML[NG][2];
+    const int b = blockIdx.y, head = blockIdx.x;
     const int ns = a.head[a.batch + b];
     if (ns <= 1) return;
     const int h = head / a.G, in = head - h * a.G, rb = in / 16, q = in - rb * 16;
     const int per = a.Hkv * a.rbs;
-    const int64_t item0 = (int64_t)a.head[b] + rb * a.Hkv + h;
-    float mt = -INFINITY;
+    const int64_t row0 = ((int64_t)a.head[b] + rb * a.Hkv + h) * 16 + q, step = (int64_t)per * 16;
+    const int grp = threadIdx.x / LP, d = (threadIdx.x % LP) * 4, dl = min(d, a.D - 4);
+    float m = -INFINITY, l = 0.f;
     bool rejected = false;
-    for (int s = lane; s < ns; s += 64) {
-        const float *ml = a.part_ml + ((item0 + (int64_t)s * per) * 16 + q) * 2;
-        mt = fmaxf(mt, ml[0]);
-        rejected |= ml[1] < 0.f;
-    }
-#pragma unroll
-    for (int off = 32; off; off >>= 1) mt = fmaxf(mt, __shfl_xor(mt, off));
-    rejected = __any(rejected);
-    const float ms = mt == -INFINITY ? 0.f : mt;
-    float lt = 0.f;
     floatx4 o = floatx4{};
-    const int d = lane * 4;
-    for (int s0 = 0; s0 < ns; s0 += 64) {
-        float f = 0.f, lx = 0.f;
-        if (s0 + lane < ns) {
-            const float *ml = a.part_ml + ((item0 + (int64_t)(s0 + lane) * per) * 16 + q) * 2;
-            f = __builtin_amdgcn_exp2f(ml[0] - ms);
-            lx = ml[1] * f;
+    for (int s0 = grp; s0 < ns; s0 += 4 * NG) {
+        floatx4 y[4];
+        float mx[4], lx[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t row = row0 + min(s0 + j * NG, ns - 1) * step;
+            mx[j] = a.part_ml[row * 2];
+            lx[j] = a.part_ml[row * 2 + 1];
+            y[j] = *reinterpret_cast<const floatx4 *>(a.part_o + row * a.D + dl);
         }
-        lt += lx;
-        const int n = min(64, ns - s0);
-        const float *po = a.part_o + ((item0 + (int64_t)s0 * per) * 16 + q) * a.D + min(d, a.D - 4);
-        const int64_t step = (int64_t)per * 16 * a.D;
-        for (int s1 = 0; s1 < n; s1 += 4) {
-            floatx4 y[4];
+        float mn = m;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const floatx4 *>(po + min(s1 + j, n - 1) * step);
+        for (int j = 0; j < 4; ++j) {
+            rejected |= lx[j] < 0.f;
+            mn = fmaxf(mn, mx[j]);
+        }
+        const float ms = mn == -INFINITY ? 0.f : mn, alpha = __builtin_amdgcn_exp2f(m - ms);
+        m = mn;
+        l *= alpha;
+        o *= alpha;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (s1 + j >= n) break;
-                const float fs = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), s1 + j));
+        for (int j = 0; j < 4; ++j) {
+            if (s0 + j * NG >= ns) break;
+            const float f = __builtin_amdgcn_exp2f(mx[j] - ms);
+            l = fmaf(lx[j], f, l);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = fmaf(y[j][e], fs, o[e]);
-            }
+            for (int e = 0; e < 4; ++e) o[e] = fmaf(y[j][e], f, o[e]);
         }
     }
+    Os[grp][threadIdx.x % LP] = o;
+    if (d == 0) {
+        ML[grp][0] = m;
+        ML[grp][1] = l;
+    }
+    rejected = __syncthreads_or(rejected);
+    if (grp || d >= a.D) return;
 #pragma unroll
-    for (int off = 32; off; off >>= 1) lt += __shfl_xor(lt, off);
-    const bool none = rejected || lt == 0.f;
-    const float inv = none ? 0.f : 1.f / (lt * E::kPScale);
+    for (int g = 1; g < NG; ++g) m = fmaxf(m, ML[g][0]);
+    const float ms = m == -INFINITY ? 0.f : m;
+    l = 0.f;
+    o = floatx4{};
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+        const float f = __builtin_amdgcn_exp2f(ML[g][0] - ms);
+        l = fmaf(ML[g][1], f, l);
+        const floatx4 y = Os[g][threadIdx.x];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = fmaf(y[e], f, o[e]);
+    }
+    const bool none = rejected || l == 0.f;
+    const float inv = none ? 0.f : 1.f / (l * E::kPScale);
     if (none) o = floatx4{};
-    if (d < a.D) {
-        T *op = static_cast<T *>(a.out) + (int64_t)b * a.o_req + (int64_t)head * a.o_head + d;
-        if constexpr (E::kBytes == 4) {
-            *reinterpret_cast<floatx4 *>(op) = o * inv;
-        } else {
-            u32x2 y = {E::pack2(o[0] * inv, o[1] * inv), E::pack2(o[2] * inv, o[3] * inv)};
-            *reinterpret_cast<u32x2 *>(op) = y;
-        }
+    T *op = static_cast<T *>(a.out) + (int64_t)b * a.o_req + (int64_t)head * a.o_head + d;
+    if constexpr (E::kBytes == 4) {
+        *reinterpret_cast<floatx4 *>(op) = o * inv;
+    } else {
+        u32x2 y = {E::pack2(o[0] * inv, o[1] * inv), E::pack2(o[2] * inv, o[3] * inv)};
+        *reinterpret_cast<u32x2 *>(op) = y;
     }
-    if (lane == 0 && a.lse) a.lse[(int64_t)b * a.Hq + head] = none ? -INFINITY : (ms + log2f(lt)) * kPLn2;
+    if (d == 0 && a.lse) a.lse[(int64_t)b * a.Hq + head] = none ? -INFINITY : (ms + log2f(l)) * kPLn2;
+}
+template <typename E>
+static void launch_join(const PagedAttnArgs &a, hipStream_t st) {
+    const dim3 grid((unsigned)a.Hq, (unsigned)a.batch);
+    if (a.D <= 64) paged_join_kernel<E, 16><<<grid, 256, 0, st>>>(a);
+    else if (a.D <= 128) paged_join_kernel<E, 32><<<grid, 256, 0, st>>>(a);
+    else paged_join_kernel<E, 64><<<grid, 256, 0, st>>>(a);
 }
 
 // --------------------------------------------------------------------------
@@ -788,10 +809,9 @@ extern "C" int cast_paged_attn_fwd(const void *q, const void *k_pages, const voi
     const PagedKernel k = paged_kernel(dtype, head_dim, any);
     if (hipLaunchKernel(k.fn, dim3((unsigned)p.items), dim3(kPWaves * 64), args, 0, st) != hipSuccess) return CAST_ERR_HIP;
     if (p.parts) {
-        const dim3 grid((unsigned)((num_q_heads + 3) / 4), (unsigned)batch);
-        if (dtype == CAST_FP32) paged_join_kernel<PF32><<<grid, 256, 0, st>>>(a);
-        else if (dtype == CAST_FP16) paged_join_kernel<PFp16><<<grid, 256, 0, st>>>(a);
-        else paged_join_kernel<PBf16><<<grid, 256, 0, st>>>(a);
+        if (dtype == CAST_FP32) launch_join<PF32>(a, st);
+        else if (dtype == CAST_FP16) launch_join<PFp16>(a, st);
+        else launch_join<PBf16>(a, st);
         if (hipGetLastError() != hipSuccess) return CAST_ERR_HIP;
     }
     return CAST_OK;

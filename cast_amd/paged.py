@@ -33,55 +33,74 @@ import operator
 import torch
 
 from . import _lib
-from .tree_attn import _DTYPES, _as_i32, _host_side, _mask_words, _ready, _require_on, check_host_metadata
+from .tree_attn import _DTYPES, _as_i32, _host_side, _mask_words, _require_on, check_host_metadata
 
 
-def _pools(k_pages, v_pages, what):
-    """The pools' common geometry (n_pages, Hkv, page_size, D)."""
-    if k_pages.dim() != 4 or tuple(v_pages.shape) != tuple(k_pages.shape):
-        raise ValueError("k_pages and v_pages must both be [n_pages, H_kv, page_size, D]")
-    if not k_pages.is_cuda:
-        raise ValueError(f"{what} runs on the GPU: the pools must be device tensors")
-    if k_pages.dtype not in _DTYPES or v_pages.dtype != k_pages.dtype:
-        raise ValueError("the pools must share one dtype: bfloat16, float16 or float32")
-    esz = k_pages.element_size()
-    if not (_in_place(k_pages, esz) and _in_place(v_pages, esz)):
-        raise ValueError("the pools need a contiguous head dim and 16-byte aligned strides")
-    return (int(x) for x in k_pages.shape)
+class _Pools:
+    """A layer's pools as the launches need them, checked: sizes, addresses and
+    strides (K's then V's), cast_dtype, element size and device index."""
+    __slots__ = ("n_pages", "H_kv", "page_size", "D", "dtype", "code", "esz", "device", "index", "k", "v", "strides")
+
+    def __init__(self, k_pages, v_pages, what):
+        shape, dt = k_pages.shape, k_pages.dtype
+        if len(shape) != 4 or v_pages.shape != shape:
+            raise ValueError("k_pages and v_pages must both be [n_pages, H_kv, page_size, D]")
+        self.n_pages, self.H_kv, self.page_size, self.D = shape
+        self.index = k_pages.get_device()
+        if self.index < 0:
+            raise ValueError(f"{what} runs on the GPU: the pools must be device tensors")
+        if dt not in _DTYPES or v_pages.dtype is not dt:
+            raise ValueError("the pools must share one dtype: bfloat16, float16 or float32")
+        self.dtype, self.code, self.esz, self.device = dt, _DTYPES[dt], dt.itemsize, k_pages.device
+        ks, vs = k_pages.stride(), v_pages.stride()
+        self.k, self.v = k_pages.data_ptr(), v_pages.data_ptr()
+        self.strides = ks[:3] + vs[:3]
+        low = self.k | self.v | (ks[0] | ks[1] | ks[2] | vs[0] | vs[1] | vs[2]) * self.esz
+        if (ks[3] != 1 or vs[3] != 1 or low & 15) and self.n_pages:
+            raise ValueError("the pools need a contiguous head dim and 16-byte aligned strides")
+        if v_pages.get_device() != self.index:
+            _require_on(self.device, v_pages=v_pages)
 
 
-def _table(page_table, dev, batch=None):
-    """page_table as int32 rows on dev (no copy when it already is that)."""
+def _table(page_table, pools, batch=None):
+    """page_table as int32 rows on the pools' device (no copy when it already is that)."""
     t = page_table
-    if not (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.get_device() == dev.index
+    if not (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.get_device() == pools.index
             and t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] <= 1)):
-        t = _as_i32(t, dev)
+        t = _as_i32(t, pools.device)
     if t.dim() != 2 or (batch is not None and t.shape[0] != batch):
         raise ValueError("page_table must be [B, max_pages]")
     return t
 
 
-def _in_place(x, esz):
-    """Whether the kernels can address x as it lies: head dim contiguous, 16-byte aligned base and strides."""
-    return x.numel() == 0 or (_ready(x, esz) is x and not x.data_ptr() & 15)
+def _rows(name, x, heads, pools, total):
+    """Check x as [total, heads, D] rows of the pools' dtype and device and
+    return it, or a copy the kernels can address: head dim contiguous, 16-byte
+    aligned base and strides."""
+    if x.shape != (total, heads, pools.D):
+        raise ValueError(f"{name} must be [{total}, {heads}, {pools.D}]")
+    if x.dtype is not pools.dtype:
+        raise ValueError(f"{name} must have the pools' dtype {pools.dtype}")
+    if x.get_device() != pools.index:
+        _require_on(pools.device, **{name: x})
+    st = x.stride()
+    if (st[2] == 1 and not (x.data_ptr() | (st[0] | st[1]) * pools.esz) & 15) or not x.numel():
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
 
 
-def _aligned(x, esz):
-    """x, or a copy the kernels can address."""
-    return x if _in_place(x, esz) else x.clone(memory_format=torch.contiguous_format)
+def _output(name, x, heads, pools, total):
+    """Check a caller's output like _rows; it is written where it lies."""
+    if _rows(name, x, heads, pools, total) is not x:
+        raise ValueError(f"{name} needs a contiguous head dim and 16-byte aligned strides")
+    _no_overlap(name, x)
+    return x
 
 
 def _no_overlap(name, t):
     """An output whose elements share memory (an expanded tensor) cannot be written."""
     if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
         raise ValueError(f"{name} must not be an expanded tensor")
-
-
-def _rows(name, x, heads, D, dtype, total=None):
-    if x.dim() != 3 or x.shape[1:] != (heads, D) or (total is not None and x.shape[0] != total):
-        raise ValueError(f"{name} must be [{'total' if total is None else total}, {heads}, {D}]")
-    if x.dtype != dtype:
-        raise ValueError(f"{name} must have the pools' dtype {dtype}")
 
 
 def paged_append(k, v, k_pages, v_pages, page_table, seq_len, cu_q=None, *, q=None, cos=None, sin=None,
@@ -106,42 +125,41 @@ def paged_append(k, v, k_pages, v_pages, page_table, seq_len, cu_q=None, *, q=No
     request's new_len stays seq_len; ``check=True`` raises.
     """
     lib = _lib.load()
-    n_pages, H_kv, page_size, D = _pools(k_pages, v_pages, "paged_append")
-    dt, dev = k_pages.dtype, k_pages.device
-    _rows("k", k, H_kv, D, dt)
-    total = int(k.shape[0])
-    _rows("v", v, H_kv, D, dt, total)
-    _require_on(dev, v_pages=v_pages, k=k, v=v, q=q, cos=cos, sin=sin, q_out=q_out, k_out=k_out, new_len=new_len)
-    esz = k.element_size()
+    pools = _Pools(k_pages, v_pages, "paged_append")
+    H_kv, D, dev, esz = pools.H_kv, pools.D, pools.device, pools.esz
+    total = k.shape[0] if k.dim() else 0
+    k, v = _rows("k", k, H_kv, pools, total), _rows("v", v, H_kv, pools, total)
     H_q = 0
     if q is not None:
-        H_q = int(q.shape[1]) if q.dim() == 3 else 0
-        _rows("q", q, H_q, D, dt, total)
+        H_q = q.shape[1] if q.dim() == 3 else 0
+        q_in = _rows("q", q, H_q, pools, total)
         assert H_q > 0 and H_q % H_kv == 0
-        if q_out is None:
-            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format) if q_out is None else \
+            _output("q_out", q_out, H_q, pools, total)
+        q_in, q_st, q_to, qo_st = q_in.data_ptr(), q_in.stride()[:2], q_out.data_ptr(), q_out.stride()[:2]
     elif q_out is not None:
         raise ValueError("q_out without q")
-    for name, t, heads in (("q_out", q_out, H_q), ("k_out", k_out, H_kv)):
-        if t is not None:
-            _rows(name, t, heads, D, dt, total)
-            _no_overlap(name, t)
-            if not _in_place(t, esz):
-                raise ValueError(f"{name} needs a contiguous head dim and 16-byte aligned strides")
-    k, v = _aligned(k, esz), _aligned(v, esz)
-    q = None if q is None else _aligned(q, esz)
+    else:
+        q_in, q_to, q_st, qo_st = None, None, (0, 0), (0, 0)
+    k_to, ko_st = (None, (0, 0)) if k_out is None else \
+        (_output("k_out", k_out, H_kv, pools, total).data_ptr(), k_out.stride()[:2])
     rot_dim = max_pos = rope_ld = 0
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin go together")
     if cos is not None:
-        if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype is not torch.float32 or sin.dtype is not torch.float32:
             raise ValueError("cos and sin must both be float32 [max_pos, rot_dim / 2]")
-        max_pos, rot_dim = int(cos.shape[0]), 2 * int(cos.shape[1])
+        max_pos, rot_dim = cos.shape[0], 2 * cos.shape[1]
         if not 0 < rot_dim <= D or rot_dim % (32 // esz):
             raise ValueError(f"rot_dim must be a multiple of {32 // esz} up to the head dim {D}, got {rot_dim}")
-        cos, sin = _aligned(cos, 4), _aligned(sin, 4)
-        if cos.stride() != sin.stride():
+        if cos.get_device() != pools.index or sin.get_device() != pools.index:
+            _require_on(dev, cos=cos, sin=sin)
+        ld = cos.stride(0)
+        if not (cos.is_contiguous() and sin.is_contiguous()) and (
+                cos.stride() != sin.stride() or cos.stride(1) != 1 or ld % 4 or ld < rot_dim // 2):
             cos, sin = cos.contiguous(), sin.contiguous()
+        if (cos.data_ptr() | sin.data_ptr()) & 15:
+            cos, sin = cos.clone(), sin.clone()
         rope_ld = cos.stride(0) if max_pos > 1 else rot_dim // 2
         if positions is not None:
             positions = _as_i32(positions, dev)
@@ -149,9 +167,9 @@ def paged_append(k, v, k_pages, v_pages, page_table, seq_len, cu_q=None, *, q=No
                 raise ValueError(f"positions must be [{total}]")
     else:
         positions = None
-    page_table = _table(page_table, dev)
+    page_table = _table(page_table, pools)
     seq_len = _as_i32(seq_len, dev)
-    B, max_pages = (int(x) for x in page_table.shape)
+    B, max_pages = page_table.shape
     if seq_len.shape != (B,):
         raise ValueError(f"seq_len must be [{B}], one entry per page_table row")
     if cu_q is not None:
@@ -162,23 +180,23 @@ def paged_append(k, v, k_pages, v_pages, page_table, seq_len, cu_q=None, *, q=No
         raise ValueError("without cu_q every request appends one row: k must have B rows")
     if new_len is None:
         new_len = torch.empty_like(seq_len)
-    elif new_len.dtype != torch.int32 or new_len.shape != (B,) or not new_len.is_contiguous():
-        raise ValueError(f"new_len must be a contiguous int32 [{B}]")
-    status = torch.zeros(1, dtype=torch.int32, device=dev) if check else None
-    one = lambda t: (ctypes.c_void_p * 1)(t.data_ptr())
-    qs, qo, ko = (t.stride()[:2] if t is not None else (0, 0) for t in (q, q_out, k_out))
-    if total or B:
-        with _lib.on_device(dev):
-            st = lib.cast_paged_append(
-                one(k), one(v), one(k_pages), one(v_pages), 1 if total else 0, page_table.data_ptr(),
-                page_table.stride(0), max_pages, n_pages, page_size, seq_len.data_ptr(), new_len.data_ptr(), B, total,
-                _lib.ptr(cu_q), None, 0, None, _lib.ptr(q), _lib.ptr(q_out), _lib.ptr(k_out), _lib.ptr(cos),
-                _lib.ptr(sin), rope_ld, max_pos, rot_dim, int(bool(interleaved)), _lib.ptr(positions), H_q, H_kv, D,
-                *k.stride()[:2], *v.stride()[:2], *k_pages.stride()[:3], *v_pages.stride()[:3], *qs, *qo, *ko,
-                _DTYPES[dt], _lib.ptr(status), _lib.stream_of(k_pages))
-        _lib.check(st, "cast_paged_append")
+    else:
+        _require_on(dev, new_len=new_len)
+        if new_len.dtype is not torch.int32 or new_len.shape != (B,) or not new_len.is_contiguous():
+            raise ValueError(f"new_len must be a contiguous int32 [{B}]")
     if not total:
         new_len.copy_(seq_len)      # nothing to append
+        return q_out, new_len
+    status = torch.zeros(1, dtype=torch.int32, device=dev) if check else None
+    one = lambda address: ctypes.byref(ctypes.c_void_p(address))
+    with _lib.on_device(dev):
+        st = lib.cast_paged_append(
+            one(k.data_ptr()), one(v.data_ptr()), one(pools.k), one(pools.v), 1, page_table.data_ptr(),
+            page_table.stride(0), max_pages, pools.n_pages, pools.page_size, seq_len.data_ptr(), new_len.data_ptr(), B,
+            total, _lib.ptr(cu_q), None, 0, None, q_in, q_to, k_to, _lib.ptr(cos), _lib.ptr(sin), rope_ld, max_pos,
+            rot_dim, 1 if interleaved else 0, _lib.ptr(positions), H_q, H_kv, D, *k.stride()[:2], *v.stride()[:2],
+            *pools.strides, *q_st, *qo_st, *ko_st, pools.code, _lib.ptr(status), _lib.stream_of(k_pages))
+    _lib.check(st, "cast_paged_append")
     if check:
         _lib.raise_device_flags(status.item(), "paged_append")
     return q_out, new_len
@@ -211,45 +229,36 @@ def paged_attention(q, k_pages, v_pages, page_table, seq_len, sm_scale=None, *, 
     """
     lib = _lib.load()
     kv_split, window = operator.index(kv_split), operator.index(window)
-    n_pages, H_kv, page_size, D = _pools(k_pages, v_pages, "paged_attention")
-    if q.dim() != 3 or q.shape[2] != D:
-        raise ValueError(f"q must be [B, H_q, {D}], the pools' head dim")
-    B, H_q = int(q.shape[0]), int(q.shape[1])
+    pools = _Pools(k_pages, v_pages, "paged_attention")
+    H_kv, D, dev = pools.H_kv, pools.D, pools.device
+    if q.dim() != 3:
+        raise ValueError(f"q must be [B, H_q, {D}]")
+    B, H_q, _ = q.shape
     assert H_q % H_kv == 0
-    if q.dtype != k_pages.dtype:
-        raise ValueError("q and the pools must share one dtype (the cache is read in place)")
-    dev = k_pages.device
-    _require_on(dev, q=q, v_pages=v_pages, out=out, workspace=workspace)
-    if window < 0 or softcap is None or not (0 <= softcap < math.inf):
+    q = _rows("q", q, H_q, pools, B)
+    if window < 0 or not 0 <= softcap < math.inf:
         raise ValueError("window and softcap must be 0 (none) or positive")
-    esz = q.element_size()
-    q = _aligned(q, esz)
-    page_table = _table(page_table, dev, B)
+    page_table = _table(page_table, pools, B)
     seq_len = _as_i32(seq_len, dev)
     if seq_len.shape != (B,):
         raise ValueError(f"seq_len must be [{B}]")
-    if out is None:
-        out = q.new_empty((B, H_q, D))
-    else:
-        if out.shape != q.shape or out.dtype != q.dtype or not _in_place(out, esz):
-            raise ValueError("out must match q's shape and dtype with a contiguous head dim, 16-byte aligned")
-        _no_overlap("out", out)
+    out = q.new_empty((B, H_q, D)) if out is None else _output("out", out, H_q, pools, B)
     lse = q.new_empty((B, H_q), dtype=torch.float32) if return_lse else None
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(D)
-    max_pages = int(page_table.shape[1])
-    dt = _DTYPES[q.dtype]
-    status = torch.zeros(1, dtype=torch.int32, device=dev) if check else None
-    ws_bytes = _workspace_bytes(dev.index, B, max_pages, page_size, H_q, H_kv, D, window, dt, kv_split)
+    max_pages = page_table.shape[1]
+    ws_bytes = _workspace_bytes(pools.index, B, max_pages, pools.page_size, H_q, H_kv, D, window, pools.code, kv_split)
+    if workspace is not None:
+        _require_on(dev, workspace=workspace)
     if ws_bytes and (workspace is None or workspace.numel() * workspace.element_size() < ws_bytes):
         workspace = q.new_empty(ws_bytes, dtype=torch.uint8)
+    status = torch.zeros(1, dtype=torch.int32, device=dev) if check else None
     with _lib.on_device(dev):
         st = lib.cast_paged_attn_fwd(
-            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), _lib.ptr(lse), page_table.data_ptr(),
-            page_table.stride(0), max_pages, n_pages, page_size, seq_len.data_ptr(), B, H_q, H_kv, D, *q.stride()[:2],
-            *k_pages.stride()[:3], *v_pages.stride()[:3], *out.stride()[:2], dt, float(sm_scale), float(softcap),
-            window, kv_split, _lib.ptr(workspace) if ws_bytes else None, ws_bytes, _lib.ptr(status),
-            _lib.stream_of(q))
+            q.data_ptr(), pools.k, pools.v, out.data_ptr(), _lib.ptr(lse), page_table.data_ptr(), page_table.stride(0),
+            max_pages, pools.n_pages, pools.page_size, seq_len.data_ptr(), B, H_q, H_kv, D, *q.stride()[:2],
+            *pools.strides, *out.stride()[:2], pools.code, float(sm_scale), float(softcap), window, kv_split,
+            workspace.data_ptr() if ws_bytes else None, ws_bytes, _lib.ptr(status), _lib.stream_of(q))
     _lib.check(st, "cast_paged_attn_fwd")
     if check:
         _lib.raise_device_flags(status.item(), "paged_attention")
@@ -299,58 +308,49 @@ def paged_tree_attention(q, k_pages, v_pages, page_table, k_pack, v_pack, cu_q, 
     """
     lib = _lib.load()
     kv_split = operator.index(kv_split)
-    n_pages, H_kv, page_size, D = _pools(k_pages, v_pages, "paged_tree_attention")
-    if n_pages == 0:
+    pools = _Pools(k_pages, v_pages, "paged_tree_attention")
+    H_kv, D, dev = pools.H_kv, pools.D, pools.device
+    if pools.n_pages == 0:
         raise ValueError("the pools must hold at least one page")
-    if q.dim() != 3 or q.shape[2] != D:
-        raise ValueError(f"q must be [total_q, H_q, {D}], the pools' head dim")
-    total_q, H_q = int(q.shape[0]), int(q.shape[1])
+    if q.dim() != 3:
+        raise ValueError(f"q must be [total_q, H_q, {D}]")
+    total_q, H_q, _ = q.shape
     assert H_q % H_kv == 0
-    if tuple(k_pack.shape) != (H_kv, total_q, D) or tuple(v_pack.shape) != (H_kv, total_q, D):
+    q = _rows("q", q, H_q, pools, total_q)
+    if k_pack.dim() != 3 or v_pack.dim() != 3:
         raise ValueError(f"k_pack/v_pack must be [{H_kv}, {total_q}, {D}]")
-    if any(t.dtype != k_pages.dtype for t in (q, k_pack, v_pack)):
-        raise ValueError("q, the pools and the pack K/V must share one dtype (the cache is read in place)")
-    dev = k_pages.device
-    _require_on(dev, q=q, v_pages=v_pages, k_pack=k_pack, v_pack=v_pack, out=out, workspace=workspace)
-    esz = q.element_size()
-    q, k_pack, v_pack = _aligned(q, esz), _aligned(k_pack, esz), _aligned(v_pack, esz)
-    page_table = _table(page_table, dev)
-    B, max_pages = (int(x) for x in page_table.shape)
-    if page_size % 64 and max_pages > 1:
+    kn = _rows("k_pack (token-major)", k_pack.transpose(0, 1), H_kv, pools, total_q)
+    vn = _rows("v_pack (token-major)", v_pack.transpose(0, 1), H_kv, pools, total_q)
+    page_table = _table(page_table, pools)
+    B, max_pages = page_table.shape
+    if pools.page_size % 64 and max_pages > 1:
         raise ValueError("paged_tree_attention needs a page size that is a multiple of 64")
-    if total_kv is None:
-        total_kv = B * max_pages * page_size + total_q
-    total_kv = operator.index(total_kv)
+    total_kv = B * max_pages * pools.page_size + total_q if total_kv is None else operator.index(total_kv)
     if not 0 <= total_kv < 1 << 31:
         raise ValueError("total_kv must be a bound on the summed lengths below 2^31")
     mask, words = _mask_words(ancestor_mask, total_q, dev)
     if _host_side(cu_q, prefix_len, pack_len):
-        check_host_metadata(cu_q, prefix_len, pack_len, total_q, total_kv, words, cap=max_pages * page_size)
+        check_host_metadata(cu_q, prefix_len, pack_len, total_q, total_kv, words, cap=max_pages * pools.page_size)
     cu_q, prefix_len, pack_len = _as_i32(cu_q, dev), _as_i32(prefix_len, dev), _as_i32(pack_len, dev)
-    if cu_q.shape[0] != B + 1 or prefix_len.shape[0] != B or pack_len.shape[0] != B:
+    if cu_q.shape != (B + 1,) or prefix_len.shape != (B,) or pack_len.shape != (B,):
         raise ValueError("cu_q needs B+1 entries and prefix_len / pack_len B entries (B rows of page_table)")
-    if out is None:
-        out = q.new_empty((total_q, H_q, D))
-    else:
-        if out.shape != q.shape or out.dtype != q.dtype or not _in_place(out, esz):
-            raise ValueError("out must match q's shape and dtype with a contiguous head dim, 16-byte aligned")
-        _no_overlap("out", out)
+    out = q.new_empty((total_q, H_q, D)) if out is None else _output("out", out, H_q, pools, total_q)
     lse = q.new_empty((total_q, H_q), dtype=torch.float32) if return_lse else None
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(D)
-    dt = _DTYPES[q.dtype]
-    ws_bytes = _tree_workspace_bytes(dev.index, B, total_q, total_kv, H_q, H_kv, D, dt, kv_split)
+    ws_bytes = _tree_workspace_bytes(pools.index, B, total_q, total_kv, H_q, H_kv, D, pools.code, kv_split)
+    if workspace is not None:
+        _require_on(dev, workspace=workspace)
     if workspace is None or workspace.numel() * workspace.element_size() < ws_bytes:
         workspace = q.new_empty(ws_bytes, dtype=torch.uint8)
     status = torch.zeros(1, dtype=torch.int32, device=dev) if check else None
     with _lib.on_device(dev):
         st = lib.cast_tree_attn_paged_fwd(
-            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), page_table.stride(0), max_pages,
-            n_pages, page_size, k_pack.data_ptr(), v_pack.data_ptr(), out.data_ptr(), _lib.ptr(lse), cu_q.data_ptr(),
+            q.data_ptr(), pools.k, pools.v, page_table.data_ptr(), page_table.stride(0), max_pages, pools.n_pages,
+            pools.page_size, kn.data_ptr(), vn.data_ptr(), out.data_ptr(), _lib.ptr(lse), cu_q.data_ptr(),
             prefix_len.data_ptr(), pack_len.data_ptr(), mask.data_ptr(), words, B, total_q, total_kv, H_q, H_kv, D,
-            *q.stride()[:2], *k_pages.stride()[:3], *v_pages.stride()[:3], *k_pack.stride()[1::-1],
-            *v_pack.stride()[1::-1], *out.stride()[:2], dt, float(sm_scale), kv_split, workspace.data_ptr(), ws_bytes,
-            _lib.ptr(status), _lib.stream_of(q))
+            *q.stride()[:2], *pools.strides, *kn.stride()[:2], *vn.stride()[:2], *out.stride()[:2], pools.code,
+            float(sm_scale), kv_split, workspace.data_ptr(), ws_bytes, _lib.ptr(status), _lib.stream_of(q))
     _lib.check(st, "cast_tree_attn_paged_fwd")
     if check:
         _lib.raise_device_flags(status.item(), "paged_tree_attention")
