@@ -18,8 +18,11 @@
 // tiles); its four waves take 16 KB of keys in turn, each on its own with its
 // own running maximum and sum, and join through LDS at the end.  No operand
 // goes through LDS:
-//   S^T = K Q^T   a lane holds 16-byte chunks of one key's row, as the
-//                 product's K-side operand wants them;
+//   S^T = K Q^T   the operand's lane (key, g) wants chunks 4 c + g of its key's
+//                 row, 64 bytes of 16 rows at a time; loaded like that, every
+//                 128-byte line is asked for twice.  A load takes 128 bytes of
+//                 8 rows instead, and a DPP move a register trades the halves
+//                 of two of them;
 //   O^T += V^T P^T  a lane holds D/16 elements of 8 keys (16-byte chunks,
 //                 neighbouring lanes reading neighbouring chunks of a row),
 //                 which v_perm turns into 8 keys of each element; the keys it
@@ -85,6 +88,11 @@ __device__ __forceinline__ float quad_max(float x) {
 __device__ __forceinline__ float quad_sum(float x) {
     x += __shfl_xor(x, 16);
     return x + __shfl_xor(x, 32);
+}
+
+// 16 bytes that this kernel reads once: not kept in the caches.
+__device__ __forceinline__ u32x4 stream16(const char *p) {
+    return __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p));
 }
 
 // ---- formats
@@ -154,7 +162,8 @@ __global__ __launch_bounds__(kPWaves * 64) void paged_attn_kernel(PagedAttnArgs 
     constexpr int KB = E::kBlocks;                 // 16-key blocks of a wave's tile
     constexpr int WK = 16 * KB;                    // keys of a wave's tile
     constexpr int TK = WK * kPWaves;               // keys of a workgroup's tile
-    constexpr int KC = F32 ? D / 16 : D / 32;      // 16-byte chunks of a key a lane holds (16 lanes hold a row's 4)
+    constexpr int KC = F32 ? D / 16 : D / 32;      // 16-byte chunks of K a lane holds
+    constexpr int KE = 16 / E::kBytes;             // elements of such a chunk
     constexpr int EPC = F32 || D == 64 ? 4 : 8;    // elements of a V chunk
     constexpr int VC = D / (16 * EPC);             // V chunks of a key a lane holds
     constexpr int VK = 4 * KB;                     // keys a lane holds V of
@@ -163,7 +172,7 @@ __global__ __launch_bounds__(kPWaves * 64) void paged_attn_kernel(PagedAttnArgs 
     __shared__ __attribute__((aligned(16))) float Os[kPWaves][16][OP];
     __shared__ float ML[kPWaves][16][2];
 
-    const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, l8 = lane & 7, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int dr = PAD ? a.D : D;
 
@@ -257,20 +266,24 @@ __global__ __launch_bounds__(kPWaves * 64) void paged_attn_kernel(PagedAttnArgs 
 #pragma unroll
         for (int t16 = 0; t16 < KB; ++t16) {
             const int kb = kt + 16 * t16;
-            // this lane's K row, and the page and offset of its four V rows
-            const char *kp, *vp[4];
+            // this lane's two K rows, and its four V rows
+            const char *kp[2], *vp[4];
             if constexpr (!ANY) {
                 // (visible keys of a block share a page; keys outside are clamped into them)
                 const int p0 = (int)((uint32_t)seen(kb) / ps * ps);
                 const int64_t id = __builtin_amdgcn_readlane(ids, (i % (64 / KB)) * KB + t16);
-                kp = kbase + id * a.kp_page + (int64_t)(seen(kb + l16) - p0) * a.kp_tok;
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+                    kp[x] = kbase + id * a.kp_page + (int64_t)(seen(kb + 8 * x + l8) - p0) * a.kp_tok;
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
                     vp[r] = vbase + id * a.vp_page + (int64_t)(seen(kb + 4 * g + r) - p0) * a.vp_tok;
             } else {
                 const int key = seen(kb + l16);
                 const int id = page_id(key), off = (int)((uint32_t)key % ps);
-                kp = kbase + (int64_t)id * a.kp_page + (int64_t)off * a.kp_tok;
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+                    kp[x] = kbase + (int64_t)__shfl(id, 8 * x + l8) * a.kp_page + (int64_t)__shfl(off, 8 * x + l8) * a.kp_tok;
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
                     vp[r] = vbase + (int64_t)__shfl(id, 4 * g + r) * a.vp_page + (int64_t)__shfl(off, 4 * g + r) * a.vp_tok;
@@ -282,19 +295,19 @@ __global__ __launch_bounds__(kPWaves * 64) void paged_attn_kernel(PagedAttnArgs 
                     const int d = (c * 16 + l16) * EPC;
                     const char *x = vp[r] + (PAD ? min(d, dr - EPC) : d) * E::kBytes;
                     if constexpr (VW == 4) {
-                        const u32x4 y = *reinterpret_cast<const u32x4 *>(x);
+                        const u32x4 y = stream16(x);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) t.v[4 * t16 + r][c][e] = y[e];
                     } else {
-                        const u32x2 y = *reinterpret_cast<const u32x2 *>(x);
+                        const u32x2 y = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(x));
                         t.v[4 * t16 + r][c][0] = y[0];
                         t.v[4 * t16 + r][c][1] = y[1];
                     }
                 }
 #pragma unroll
             for (int c = 0; c < KC; ++c) {
-                const int d = F32 ? c * 16 + g * 4 : c * 32 + g * 8;
-                t.k[t16][c] = *reinterpret_cast<const u32x4 *>(kp + (PAD ? min(d, dr - 16 / E::kBytes) : d) * E::kBytes);
+                const int d = ((c >> 1) * 8 + (l16 >> 3) * 4 + g) * KE;
+                t.k[t16][c] = stream16(kp[c & 1] + (PAD ? min(d, dr - KE) : d) * E::kBytes);
             }
         }
     };
@@ -310,7 +323,15 @@ __global__ __launch_bounds__(kPWaves * 64) void paged_attn_kernel(PagedAttnArgs 
             floatx4 s4 = floatx4{};
 #pragma unroll
             for (int c = 0; c < KC; ++c) {
-                u32x4 kx = t.k[t16][c];
+                // words of chunk pair (c & ~1, c | 1): the loads left the first
+                // eight keys in one register, the others in the next
+                u32x4 kx;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t near = t.k[t16][c & ~1][e], far = t.k[t16][c | 1][e];
+                    kx[e] = c & 1 ? (uint32_t)__builtin_amdgcn_update_dpp((int)far, (int)near, 0x128, 0xf, 0x3, false)
+                                  : (uint32_t)__builtin_amdgcn_update_dpp((int)near, (int)far, 0x128, 0xf, 0xc, false);
+                }
                 if constexpr (PAD) {
                     // (chunks past the head dim were read from its last one)
                     const int d = F32 ? c * 16 + g * 4 : c * 32 + g * 8;
