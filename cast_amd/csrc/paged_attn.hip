@@ -14,8 +14,8 @@
 // matrix products, so each key is read once for all of them and the products
 // cost a tenth of the time its bytes take.
 //
-// A work item is (request, KV head, block of 16 query heads, run of key
-// tiles); its four waves take 16 KB of keys in turn, each on its own with its
+// A work item is a run of key tiles of one (request, KV head, block of 16 query
+// heads); the four waves of a workgroup take 16 KB of keys in turn, each on its own with its
 // own running maximum and sum, and join through LDS at the end.  No operand
 // goes through LDS:
 //   S^T = K Q^T   the operand's lane (key, g) wants chunks 4 c + g of its key's
@@ -35,11 +35,13 @@
 // memory behind the last token may hold anything.
 //
 // The next tile's loads are issued before the current one is used; page ids
-// are loaded 64 blocks ahead.  Long requests are split over keys, each split
-// writes (O, max, sum) in float and a second kernel joins them.
+// are loaded 64 blocks ahead.  The keys of all requests are dealt out in
+// equal stretches, pieces of a request write (O, max, sum) in float and a
+// second kernel joins them.
 #include <limits.h>
 #include <math.h>
 
+#include <algorithm>
 #include <mutex>
 
 #include "cast_common.hpp"
@@ -49,7 +51,7 @@ namespace cast {
 constexpr float kPLn2 = 0.69314718055994530942f;
 constexpr float kPLog2e = 1.44269504088896340736f;
 constexpr int kPWaves = 4;
-constexpr int kMinTiles = 2;             // fewest key tiles of an automatic split
+constexpr int kMinTiles = 2;             // fewest key tiles of a workgroup's stretch, unless the caller says
 
 struct PagedAttnArgs {
     const void *q, *k, *v;
@@ -60,12 +62,14 @@ struct PagedAttnArgs {
     int64_t table_ld, q_req, q_head, o_req, o_head;                      // elements (q, out)
     int64_t kp_page, kp_head, kp_tok, vp_page, vp_head, vp_tok;          // bytes
     int32_t n_pages, page_size, batch, Hq, Hkv, G, rbs, D, cap, window;  // cap: slots a table row covers
-    int32_t split;      // tiles per split asked for; 0: chosen from the lengths; INT_MAX: one split
-    int32_t slots;      // workgroups resident at once
+    FastDiv by_page;    // division by page_size
+    int32_t wgs;        // workgroups of the attention kernel
+    int32_t least;      // fewest tiles of a run; 0: one workgroup per unit, no runs
+    int32_t prows;      // rows of a partial: min(16, G)
     float scale, softcap;   // scale: natural scale (softcap) or times log2(e)
-    int32_t *head;      // workspace: [batch] first item, [batch] splits
-    float *part_ml;     // [items][16][2] running maximum (base 2) and sum; sum < 0: a page id is bad
-    float *part_o;      // [items][16][D]
+    int32_t *head;      // workspace: all tiles, then each request's first tile
+    float *part_ml;     // [2 wgs][prows][2] running maximum (base 2) and sum; sum < 0: a page id is bad
+    float *part_o;      // [2 wgs][prows][D]
 };
 
 // ---- lanes and waves
@@ -90,10 +94,8 @@ __device__ __forceinline__ float quad_sum(float x) {
     return x + __shfl_xor(x, 32);
 }
 
-// 16 bytes that this kernel reads once: not kept in the caches.
-__device__ __forceinline__ u32x4 stream16(const char *p) {
-    return __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p));
-}
+// The cache policy of loads that this kernel does once: not kept in the caches (the nt bit).
+constexpr int kOnce = 2;
 
 // ---- formats
 struct PF32 {
@@ -120,43 +122,42 @@ struct PFp16 : Fp16 {
     }
 };
 
-// ---- the schedule, found by every workgroup from the lengths
+// ---- the schedule, found by every workgroup from the lengths.  The units
+// (request, block of 16 query heads, KV head), each a run of key tiles, lie in
+// a line, and the workgroups take equal stretches of it: with `all` tiles and
+// W workgroups, the first all % W take one tile more than the others.  A
+// workgroup walks its stretch unit by unit; a unit that it covers whole goes
+// to the output, a piece of one to a partial, of which a workgroup has at most
+// two (its first and its last).
 struct PagedReq {
-    int start, len, t0, tiles;   // visible slots [start, len), key tiles [t0, t0 + tiles)
+    int start, len, t0, tiles;   // visible slots [start, len), key tiles [t0, t0 + tiles); a tile where none is seen
 };
-template <int TK>
-__device__ __forceinline__ PagedReq paged_req(const PagedAttnArgs &a, int b, bool report) {
-    PagedReq r{0, 0, 0, 0};
-    const int len = a.seq_len[b];
-    if (len < 0 || len > a.cap) {
-        if (report) raise_flag(a.status, CAST_FLAG_BAD_OFFSETS);
-        return r;
-    }
+__device__ __forceinline__ PagedReq paged_req(const PagedAttnArgs &a, int tk, int len) {
+    PagedReq r{0, 0, 0, 1};
+    if (len <= 0 || len > a.cap) return r;
     r.len = len;
     r.start = a.window > 0 && len > a.window ? len - a.window : 0;
-    r.t0 = r.start / TK;
-    r.tiles = (len + TK - 1) / TK - r.t0;
+    r.t0 = r.start / tk;
+    r.tiles = (len + tk - 1) / tk - r.t0;
     return r;
 }
-
-// Tiles per split for the batch: an even share of the resident workgroups.
-template <int TK>
-__device__ __forceinline__ int paged_split(const PagedAttnArgs &a) {
-    if (a.split) return a.split;
-    const int lane = threadIdx.x & 63;
-    int64_t total = 0;
-    for (int b0 = 0; b0 < a.batch; b0 += 64)
-        total += p_wave_sum(b0 + lane < a.batch ? paged_req<TK>(a, b0 + lane, false).tiles : 0);
-    total *= a.Hkv * a.rbs;
-    const int64_t c = (total + a.slots - 1) / a.slots;
-    return c < kMinTiles ? kMinTiles : (int)c;
-}
-__device__ __forceinline__ int splits_of(int tiles, int split) {
-    return tiles <= split ? 1 : (int)(((uint32_t)tiles + (uint32_t)split - 1) / (uint32_t)split);
-}
+struct Stretches {
+    int W, q, r;
+    __device__ __forceinline__ Stretches(const PagedAttnArgs &a, int all) {
+        W = min(a.wgs, (int)(((uint32_t)all + (uint32_t)a.least - 1) / (uint32_t)a.least));
+        q = (int)((uint32_t)all / (uint32_t)W);
+        r = all - q * W;
+    }
+    __device__ __forceinline__ int first(int x) const { return x * q + min(x, r); }   // workgroup x's first tile
+    __device__ __forceinline__ int of(int tile) const {                               // whose tile it is
+        const int wide = r * (q + 1);
+        return tile < wide ? (int)((uint32_t)tile / (uint32_t)(q + 1)) : r + (int)((uint32_t)(tile - wide) / (uint32_t)q);
+    }
+};
 
 template <int D, typename E, bool PAD, bool ANY>
-__global__ __launch_bounds__(kPWaves * 64) void paged_attn_kernel(PagedAttnArgs a) {
+__global__ __launch_bounds__(kPWaves * 64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : (D == 128 ? 2 : 3) - ANY)))
+void paged_attn_kernel(PagedAttnArgs a) {
     using T = typename E::T;
     constexpr bool F32 = E::kBytes == 4;
     constexpr int KB = E::kBlocks;                 // 16-key blocks of a wave's tile
@@ -176,45 +177,63 @@ __global__ __launch_bounds__(kPWaves * 64) void paged_attn_kernel(PagedAttnArgs 
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int dr = PAD ? a.D : D;
 
-    // ---- this workgroup's item: items run (request, split, query block, KV head), the head fastest
-    const int split = paged_split<TK>(a);
-    const int per = a.Hkv * a.rbs;
-    int b = 0, local = 0, first = 0;
-    {
-        int at = 0;
-        bool found = false;
-        for (int b0 = 0; b0 < a.batch && !found; b0 += 64) {
-            const int bb = b0 + lane;
-            const int n = bb < a.batch ? splits_of(paged_req<TK>(a, bb, blockIdx.x == 0 && w == 0).tiles, split) * per : 0;
+    // ---- this workgroup's stretch [p, p_end) of tiles; lane j knows the
+    // length of request b0 + j, whose tiles start at `base` for request b
+    const int per = a.Hkv * a.rbs, x = blockIdx.x;
+    int b0 = 0, b = 0, base = 0, p = 0, p_first = 0, p_end = 0, len_l = 0;
+    if (a.least) {
+        int all = 0;
+        for (int c = 0; c < a.batch; c += 64) {
+            const int bb = c + lane;
+            const int len = bb < a.batch ? a.seq_len[bb] : 0;
+            const int n = bb < a.batch ? paged_req(a, TK, len).tiles * per : 0;
             const int incl = p_wave_scan(n);
-            const uint64_t past = __ballot(at + incl <= (int)blockIdx.x);
-            const int k = __popcll(past);
-            if (k < 64) {
-                found = true;
-                b = b0 + k;
-                first = at + __builtin_amdgcn_readlane(incl - n, k);
-                local = (int)blockIdx.x - first;
+            if (x == 0 && w == 0 && bb < a.batch) {
+                a.head[1 + bb] = all + incl - n;
+                if (len < 0 || len > a.cap) raise_flag(a.status, CAST_FLAG_BAD_OFFSETS);
             }
-            at += __builtin_amdgcn_readlane(incl, 63);
+            all += __builtin_amdgcn_readlane(incl, 63);
+            len_l = len;
         }
-        // (workgroup 0 finds its item in the first 64 requests; the rest are checked all the same)
-        if (blockIdx.x == 0 && w == 0)
-            for (int bb = 64 + lane; bb < a.batch; bb += 64) paged_req<TK>(a, bb, true);
-        if (!found || b >= a.batch) return;
+        if (x == 0 && tid == 0) a.head[0] = all;
+        const Stretches st(a, all);
+        if (x >= st.W) return;
+        p_first = p = st.first(x);
+        p_end = st.first(x + 1);
+        for (;; b0 += 64) {
+            if (a.batch > 64) len_l = b0 + lane < a.batch ? a.seq_len[b0 + lane] : 0;
+            const int n = b0 + lane < a.batch ? paged_req(a, TK, len_l).tiles * per : 0;
+            const int incl = p_wave_scan(n);
+            const uint64_t past = __ballot(base + incl <= p);
+            if (~past) {
+                const int k = __builtin_ctzll(~past);
+                b = b0 + k;
+                base += __builtin_amdgcn_readlane(incl - n, k);
+                break;
+            }
+            base += __builtin_amdgcn_readlane(incl, 63);
+        }
+    } else {
+        b = (int)((uint32_t)x / (uint32_t)per);
+        b0 = b;
+        len_l = a.seq_len[b];
+        const int tiles = paged_req(a, TK, __builtin_amdgcn_readfirstlane(len_l)).tiles;
+        p_first = p = (x - b * per) * tiles;
+        p_end = p + tiles;
+        if (x == b * per && tid == 0 && (len_l < 0 || len_l > a.cap)) raise_flag(a.status, CAST_FLAG_BAD_OFFSETS);
     }
-    const PagedReq rq = paged_req<TK>(a, b, false);
-    const int ns = splits_of(rq.tiles, split);
-    const int s = local / per, rest = local - s * per;
-    const int rb = rest / a.Hkv, h = rest - rb * a.Hkv;
-    if (ns > 1 && local == 0 && tid == 0) {
-        a.head[b] = first;
-        a.head[a.batch + b] = ns;
-    } else if (ns == 1 && a.head && local == 0 && tid == 0) {
-        a.head[a.batch + b] = 1;
-    }
-    // even splits: tiles [s, s + 1) * tiles / ns
-    const int ta = (int)((int64_t)rq.tiles * s / ns), tb = (int)((int64_t)rq.tiles * (s + 1) / ns);
-    const int nt = tb - ta;
+    for (;;) {
+    // (wave-uniform all along; told so, that addresses stay scalar)
+    p = __builtin_amdgcn_readfirstlane(p);
+    p_end = __builtin_amdgcn_readfirstlane(p_end);
+    base = __builtin_amdgcn_readfirstlane(base);
+    b = __builtin_amdgcn_readfirstlane(b);
+    b0 = __builtin_amdgcn_readfirstlane(b0);
+    const PagedReq rq = paged_req(a, TK, __builtin_amdgcn_readlane(len_l, b - b0));
+    const int unit = (int)((uint32_t)(p - base) / (uint32_t)rq.tiles), ta = p - base - unit * rq.tiles;
+    const int nt = min(p_end - p, rq.tiles - ta);  // tiles of this piece
+    const bool whole = nt == rq.tiles;
+    const int rb = unit / a.Hkv, h = unit - rb * a.Hkv;
     const int key0 = (rq.t0 + ta) * TK + w * WK;   // the wave's first key
     const int rows = min(16, a.G - rb * 16);       // query heads of this block
     const int hq = h * a.G + rb * 16 + l16;
@@ -243,10 +262,9 @@ __global__ __launch_bounds__(kPWaves * 64) void paged_attn_kernel(PagedAttnArgs 
     const char *kbase = static_cast<const char *>(a.k) + (int64_t)h * a.kp_head;
     const char *vbase = static_cast<const char *>(a.v) + (int64_t)h * a.vp_head;
     const int32_t *row = a.table + (int64_t)b * a.table_ld;
-    const uint32_t ps = (uint32_t)a.page_size;
     auto seen = [&](int key) __attribute__((always_inline)) { return min(max(key, rq.start), rq.len - 1); };
     auto page_id = [&](int key) __attribute__((always_inline)) {   // of a visible key; always a page of the pool
-        const int id = row[(uint32_t)key / ps];
+        const int id = row[a.by_page.div(key)];
         bad |= id < 0 || id >= a.n_pages;
         return min(max(id, 0), a.n_pages - 1);
     };
@@ -261,53 +279,79 @@ __global__ __launch_bounds__(kPWaves * 64) void paged_attn_kernel(PagedAttnArgs 
         uint32_t v[VK][VC][EPC * E::kBytes / 4];
     };
     constexpr int VW = EPC * E::kBytes / 4;        // 32-bit words of a V chunk
+    // Byte offsets of this lane's chunks within a 16-key block.  Without ANY
+    // they belong to a buffer resource that ends behind the block's last seen
+    // key: what lies past it, and past the head dim, loads as zeros.
+    constexpr uint32_t kNowhere = 0x7ffffff0u;
+    auto k_at = [&](int c) __attribute__((always_inline)) {
+        const int d = ((c >> 1) * 8 + (l16 >> 3) * 4 + g) * KE;
+        return PAD && d >= dr ? kNowhere : (uint32_t)(8 * (c & 1) + l8) * (uint32_t)a.kp_tok + (uint32_t)(d * E::kBytes);
+    };
+    auto v_at = [&](int r, int c) __attribute__((always_inline)) {
+        const int d = (c * 16 + l16) * EPC;
+        return PAD && d >= dr ? kNowhere : (uint32_t)(4 * g + r) * (uint32_t)a.vp_tok + (uint32_t)(d * E::kBytes);
+    };
+    auto block = [&](const char *base, int keys, int64_t tok) __attribute__((always_inline)) {
+        const int bytes = keys > 0 ? (min(keys, 16) - 1) * (int)tok + dr * E::kBytes : 0;
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, bytes, 0x00020000);
+    };
+    auto set_v = [&](Tile &t, int j, int c, auto y) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < VW; ++e) t.v[j][c][e] = y[e];
+    };
     auto load_tile = [&](Tile &t, int i) __attribute__((always_inline)) {
         const int kt = key0 + i * TK;
 #pragma unroll
         for (int t16 = 0; t16 < KB; ++t16) {
             const int kb = kt + 16 * t16;
-            // this lane's two K rows, and its four V rows
-            const char *kp[2], *vp[4];
             if constexpr (!ANY) {
-                // (visible keys of a block share a page; keys outside are clamped into them)
-                const int p0 = (int)((uint32_t)seen(kb) / ps * ps);
+                // the block's seen keys share a page
+                const int kc = seen(kb), off = kb - a.by_page.div(kc) * a.page_size;
+                const int keys = kb + 16 > rq.start ? rq.len - kb : 0;
                 const int64_t id = __builtin_amdgcn_readlane(ids, (i % (64 / KB)) * KB + t16);
+                const __amdgpu_buffer_rsrc_t kr = block(kbase + id * a.kp_page + off * a.kp_tok, keys, a.kp_tok);
+                const __amdgpu_buffer_rsrc_t vr = block(vbase + id * a.vp_page + off * a.vp_tok, keys, a.vp_tok);
 #pragma unroll
-                for (int x = 0; x < 2; ++x)
-                    kp[x] = kbase + id * a.kp_page + (int64_t)(seen(kb + 8 * x + l8) - p0) * a.kp_tok;
+                for (int c = 0; c < KC; ++c)
+                    t.k[t16][c] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(kr, (int)k_at(c), 0, kOnce));
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    vp[r] = vbase + id * a.vp_page + (int64_t)(seen(kb + 4 * g + r) - p0) * a.vp_tok;
+#pragma unroll
+                    for (int c = 0; c < VC; ++c) {
+                        if constexpr (VW == 4)
+                            set_v(t, 4 * t16 + r, c, __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(vr, (int)v_at(r, c), 0, kOnce)));
+                        else
+                            set_v(t, 4 * t16 + r, c, __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(vr, (int)v_at(r, c), 0, kOnce)));
+                    }
             } else {
+                // every key's own page; keys that are not seen are clamped into those that are
                 const int key = seen(kb + l16);
-                const int id = page_id(key), off = (int)((uint32_t)key % ps);
+                const int id = page_id(key), off = key - a.by_page.div(key) * a.page_size;
+                auto row_at = [&](const char *pool, int64_t page, int64_t tok, int from) __attribute__((always_inline)) {
+                    return pool + (int64_t)__shfl(id, from) * page + (int64_t)__shfl(off, from) * tok;
+                };
 #pragma unroll
-                for (int x = 0; x < 2; ++x)
-                    kp[x] = kbase + (int64_t)__shfl(id, 8 * x + l8) * a.kp_page + (int64_t)__shfl(off, 8 * x + l8) * a.kp_tok;
+                for (int y = 0; y < 2; ++y) {
+                    const char *kp = row_at(kbase, a.kp_page, a.kp_tok, 8 * y + l8);
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    vp[r] = vbase + (int64_t)__shfl(id, 4 * g + r) * a.vp_page + (int64_t)__shfl(off, 4 * g + r) * a.vp_tok;
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-                for (int c = 0; c < VC; ++c) {
-                    const int d = (c * 16 + l16) * EPC;
-                    const char *x = vp[r] + (PAD ? min(d, dr - EPC) : d) * E::kBytes;
-                    if constexpr (VW == 4) {
-                        const u32x4 y = stream16(x);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) t.v[4 * t16 + r][c][e] = y[e];
-                    } else {
-                        const u32x2 y = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(x));
-                        t.v[4 * t16 + r][c][0] = y[0];
-                        t.v[4 * t16 + r][c][1] = y[1];
+                    for (int c = y; c < KC; c += 2) {
+                        const int d = ((c >> 1) * 8 + (l16 >> 3) * 4 + g) * KE;
+                        const u32x4 z = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(kp + min(d, dr - KE) * E::kBytes));
+                        t.k[t16][c] = d < dr ? z : u32x4{};
                     }
                 }
 #pragma unroll
-            for (int c = 0; c < KC; ++c) {
-                const int d = ((c >> 1) * 8 + (l16 >> 3) * 4 + g) * KE;
-                t.k[t16][c] = stream16(kp[c & 1] + (PAD ? min(d, dr - KE) : d) * E::kBytes);
+                for (int r = 0; r < 4; ++r) {
+                    const char *vp = row_at(vbase, a.vp_page, a.vp_tok, 4 * g + r);
+#pragma unroll
+                    for (int c = 0; c < VC; ++c) {
+                        const char *from = vp + min((c * 16 + l16) * EPC, dr - EPC) * E::kBytes;
+                        if constexpr (VW == 4)
+                            set_v(t, 4 * t16 + r, c, __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(from)));
+                        else
+                            set_v(t, 4 * t16 + r, c, __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(from)));
+                    }
+                }
             }
         }
     };
@@ -317,6 +361,7 @@ __global__ __launch_bounds__(kPWaves * 64) void paged_attn_kernel(PagedAttnArgs 
         const int kt = key0 + i * TK;
         const bool edge = kt < rq.start || kt + WK > rq.len;
         float p[KB][4];
+        __builtin_amdgcn_sched_barrier(0);   // (in this order: a tile's registers, not two stages')
         // ---- scores, base 2
 #pragma unroll
         for (int t16 = 0; t16 < KB; ++t16) {
@@ -331,11 +376,6 @@ __global__ __launch_bounds__(kPWaves * 64) void paged_attn_kernel(PagedAttnArgs 
                     const uint32_t near = t.k[t16][c & ~1][e], far = t.k[t16][c | 1][e];
                     kx[e] = c & 1 ? (uint32_t)__builtin_amdgcn_update_dpp((int)far, (int)near, 0x128, 0xf, 0x3, false)
                                   : (uint32_t)__builtin_amdgcn_update_dpp((int)near, (int)far, 0x128, 0xf, 0xc, false);
-                }
-                if constexpr (PAD) {
-                    // (chunks past the head dim were read from its last one)
-                    const int d = F32 ? c * 16 + g * 4 : c * 32 + g * 8;
-                    if (d >= dr) kx = u32x4{};
                 }
                 if constexpr (F32) {
 #pragma unroll
@@ -373,10 +413,13 @@ __global__ __launch_bounds__(kPWaves * 64) void paged_attn_kernel(PagedAttnArgs 
                     const int key = kt + 16 * t16 + 4 * g + r;
                     if (key < rq.start || key >= rq.len) {
                         p[t16][r] = -INFINITY;
+                        // (rows past the last key were loaded as zeros)
+                        if (ANY || key < rq.start) {
 #pragma unroll
-                        for (int c = 0; c < VC; ++c)
+                            for (int c = 0; c < VC; ++c)
 #pragma unroll
-                            for (int e = 0; e < VW; ++e) t.v[4 * t16 + r][c][e] = 0u;
+                                for (int e = 0; e < VW; ++e) t.v[4 * t16 + r][c][e] = 0u;
+                        }
                     }
                 }
         }
@@ -403,6 +446,7 @@ __global__ __launch_bounds__(kPWaves * 64) void paged_attn_kernel(PagedAttnArgs 
                 l += p[t16][r];
             }
         // ---- O^T += V^T P^T
+        __builtin_amdgcn_sched_barrier(0);
         if constexpr (F32) {
 #pragma unroll
             for (int r = 0; r < 4; ++r)
@@ -445,13 +489,14 @@ __global__ __launch_bounds__(kPWaves * 64) void paged_attn_kernel(PagedAttnArgs 
                     const auto vv = __builtin_bit_cast(typename E::vec8, vx);
                     acc[c * EPC + e] = E::mma16(vv, __builtin_bit_cast(typename E::vec8, hi), acc[c * EPC + e]);
                     acc[c * EPC + e] = E::mma16(vv, __builtin_bit_cast(typename E::vec8, lo), acc[c * EPC + e]);
+                    if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
                 }
         }
     };
 
     // where the wave's O^T lies in its part of the join's LDS
     auto place = [&](int c, int r) __attribute__((always_inline)) { return &Os[w][l16][(c * 16 + 4 * g + r) * EPC]; };
-    if (nt > 0) {
+    if (rq.len > 0) {
         for (;;) {
             Tile buf[2];
             if constexpr (!ANY) load_ids(0);
@@ -516,22 +561,22 @@ __global__ __launch_bounds__(kPWaves * 64) void paged_attn_kernel(PagedAttnArgs 
         float mt = -INFINITY, lt = 0.f;
         bool rejected = false;
 #pragma unroll
-        for (int x = 0; x < kPWaves; ++x) mt = fmaxf(mt, ML[x][q][0]);
+        for (int y = 0; y < kPWaves; ++y) mt = fmaxf(mt, ML[y][q][0]);
         const float ms = mt == -INFINITY ? 0.f : mt;
         floatx4 o = floatx4{};
 #pragma unroll
-        for (int x = 0; x < kPWaves; ++x) {
-            const float f = __builtin_amdgcn_exp2f(ML[x][q][0] - ms), lx = ML[x][q][1];
+        for (int wv = 0; wv < kPWaves; ++wv) {
+            const float f = __builtin_amdgcn_exp2f(ML[wv][q][0] - ms), lx = ML[wv][q][1];
             rejected |= lx < 0.f;
             lt = fmaf(lx, f, lt);
-            const floatx4 y = *reinterpret_cast<const floatx4 *>(&Os[x][q][d]);
+            const floatx4 y = *reinterpret_cast<const floatx4 *>(&Os[wv][q][d]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[e] = fmaf(y[e], f, o[e]);
         }
         if (rejected && u == 0) raise_flag(a.status, CAST_FLAG_BAD_PAGE);
         const int head = h * a.G + rb * 16 + q;
-        if (ns > 1) {
-            const int64_t at = (int64_t)blockIdx.x * 16 + q;
+        if (!whole) {
+            const int64_t at = (int64_t)(2 * x + (p != p_first)) * a.prows + q;
             *reinterpret_cast<floatx4 *>(a.part_o + at * dr + d) = o;
             if (d == 0) {
                 a.part_ml[at * 2] = mt;
@@ -551,23 +596,39 @@ __global__ __launch_bounds__(kPWaves * 64) void paged_attn_kernel(PagedAttnArgs 
                 a.lse[(int64_t)b * a.Hq + head] = rejected || lt == 0.f ? -INFINITY : (ms + log2f(lt)) * kPLn2;
         }
     }
+    // ---- the next piece
+    p += nt;
+    if (p >= p_end) return;
+    if (p == base + rq.tiles * per) {
+        base = p;
+        if (++b == b0 + 64) {
+            b0 = b;
+            len_l = b0 + lane < a.batch ? a.seq_len[b0 + lane] : 0;
+        }
+    }
+    __syncthreads();   // (the join's LDS is read)
+    }
 }
 
-// Joins the splits of one (request, query head): groups of LP lanes, one
+// Joins the pieces of one (request, query head): groups of LP lanes, one
 // float4 of the head dim a lane, walk every NG-th split with up to four in
 // flight and their own running maximum, then join through LDS.
 template <typename E, int LP>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int tk) {
     using T = typename E::T;
     constexpr int NG = 256 / LP;
     __shared__ __attribute__((aligned(16))) floatx4 Os[NG][LP];
     __shared__ float ML[NG][2];
     const int b = blockIdx.y, head = blockIdx.x;
-    const int ns = a.head[a.batch + b];
-    if (ns <= 1) return;
+    const PagedReq rq = paged_req(a, tk, a.seq_len[b]);
     const int h = head / a.G, in = head - h * a.G, rb = in / 16, q = in - rb * 16;
-    const int per = a.Hkv * a.rbs;
-    const int64_t row0 = ((int64_t)a.head[b] + rb * a.Hkv + h) * 16 + q, step = (int64_t)per * 16;
+    const Stretches st(a, a.head[0]);
+    const int first = a.head[1 + b] + (rb * a.Hkv + h) * rq.tiles;
+    const int x0 = st.of(first), ns = st.of(first + rq.tiles - 1) - x0 + 1;
+    if (ns <= 1) return;
+    // the first piece is its workgroup's last one, unless the unit starts there
+    const int late = st.first(x0) != first;
+    auto row_of = [&](int s) __attribute__((always_inline)) { return (int64_t)(2 * (x0 + s) + (s == 0 ? late : 0)) * a.prows + q; };
     const int grp = threadIdx.x / LP, d = (threadIdx.x % LP) * 4, dl = min(d, a.D - 4);
     float m = -INFINITY, l = 0.f;
     bool rejected = false;
@@ -577,7 +638,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
         float mx[4], lx[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int64_t row = row0 + min(s0 + j * NG, ns - 1) * step;
+            const int64_t row = row_of(min(s0 + j * NG, ns - 1));
             mx[j] = a.part_ml[row * 2];
             lx[j] = a.part_ml[row * 2 + 1];
             y[j] = *reinterpret_cast<const floatx4 *>(a.part_o + row * a.D + dl);
@@ -634,11 +695,11 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
     if (d == 0 && a.lse) a.lse[(int64_t)b * a.Hq + head] = none ? -INFINITY : (ms + log2f(l)) * kPLn2;
 }
 template <typename E>
-static void launch_join(const PagedAttnArgs &a, hipStream_t st) {
+static void launch_join(const PagedAttnArgs &a, int tk, hipStream_t st) {
     const dim3 grid((unsigned)a.Hq, (unsigned)a.batch);
-    if (a.D <= 64) paged_join_kernel<E, 16><<<grid, 256, 0, st>>>(a);
-    else if (a.D <= 128) paged_join_kernel<E, 32><<<grid, 256, 0, st>>>(a);
-    else paged_join_kernel<E, 64><<<grid, 256, 0, st>>>(a);
+    if (a.D <= 64) paged_join_kernel<E, 16><<<grid, 256, 0, st>>>(a, tk);
+    else if (a.D <= 128) paged_join_kernel<E, 32><<<grid, 256, 0, st>>>(a, tk);
+    else paged_join_kernel<E, 64><<<grid, 256, 0, st>>>(a, tk);
 }
 
 // --------------------------------------------------------------------------
@@ -698,42 +759,34 @@ static int paged_slots(const PagedKernel &k) {
 }
 
 struct PagedPlan {
-    int32_t split;      // as PagedAttnArgs
-    int32_t slots;
-    int64_t items;      // workgroups, an upper bound for any lengths
-    bool parts;         // whether a request may be split
+    int32_t wgs, least;   // as PagedAttnArgs
+    bool fits;            // tile indices fit 31 bits for any lengths
 };
 static PagedPlan paged_plan(int32_t batch, int32_t max_pages, int32_t page_size, int32_t Hq, int32_t Hkv, int32_t D,
                             int32_t window, int32_t dtype, int32_t kv_split) {
     const PagedKernel k = paged_kernel(dtype, D, paged_any(page_size, max_pages));
-    PagedPlan p{};
-    p.slots = paged_slots(k);
-    const int64_t per = (int64_t)Hkv * ((Hq / Hkv + 15) / 16);
+    const int64_t units = (int64_t)batch * Hkv * ((Hq / Hkv + 15) / 16);
     int64_t keys = (int64_t)max_pages * page_size;
     if (window > 0 && window < keys) keys = (int64_t)window + k.tile - 1;   // (a window may start inside a tile)
     const int64_t tiles = (keys + k.tile - 1) / k.tile;
-    int64_t least = kMinTiles;
-    if (kv_split > 0) {
-        p.split = (int32_t)(((int64_t)kv_split + k.tile - 1) / k.tile);
-        least = p.split;
-    } else if (kv_split < 0) {
-        p.split = INT_MAX;
-        least = INT_MAX;
-    }
-    const int64_t most = tiles <= least ? 1 : (tiles + least - 1) / least;   // splits of one request
-    p.parts = most > 1;
-    if (!p.parts) p.split = INT_MAX;
-    p.items = batch * per * most;
-    // an automatic split of c tiles, c * slots >= all tiles, makes at most
-    // slots + one item per unit
-    if (kv_split == 0 && p.parts && p.items > p.slots + batch * per) p.items = p.slots + batch * per;
-    return p;
+    const int64_t least = kv_split > 0 ? ((int64_t)kv_split + k.tile - 1) / k.tile : kMinTiles;
+    if (kv_split < 0 || tiles <= least) return {units > INT_MAX ? 0 : (int32_t)units, 0, units <= INT_MAX};
+    if (units > INT_MAX / tiles) return {0, 0, false};
+    const int64_t most = (units * tiles + least - 1) / least;
+    const int64_t wgs = kv_split > 0 ? most : std::min<int64_t>(most, paged_slots(k));
+    return {(int32_t)wgs, (int32_t)least, true};
 }
 static size_t p_align256(size_t x) { return (x + 255) & ~(size_t)255; }
-static size_t paged_ws(const PagedPlan &p, int32_t batch, int32_t D) {
-    if (!p.parts) return 0;
-    return p_align256((size_t)batch * 2 * sizeof(int32_t)) + p_align256((size_t)p.items * 16 * 2 * sizeof(float)) +
-           p_align256((size_t)p.items * 16 * D * sizeof(float));
+struct PagedParts {
+    size_t ml, o, all;   // offsets of the partials' sums and outputs, bytes in all
+};
+static PagedParts paged_parts(const PagedPlan &p, int32_t batch, int32_t G, int32_t D) {
+    const size_t rows = (size_t)2 * p.wgs * std::min(G, 16);
+    PagedParts s{};
+    s.ml = p_align256(((size_t)batch + 1) * sizeof(int32_t));
+    s.o = s.ml + p_align256(rows * 2 * sizeof(float));
+    s.all = p.least ? s.o + p_align256(rows * D * sizeof(float)) : 0;
+    return s;
 }
 
 }  // namespace cast
@@ -747,8 +800,8 @@ extern "C" size_t cast_paged_attn_workspace_size(int32_t batch, int32_t max_page
         num_q_heads % num_kv_heads || head_dim <= 0 || head_dim % 8 || head_dim > 256)
         return 0;
     if (dtype != CAST_BF16 && dtype != CAST_FP16 && dtype != CAST_FP32) return 0;
-    return paged_ws(paged_plan(batch, max_pages, page_size, num_q_heads, num_kv_heads, head_dim, window, dtype, kv_split),
-                    batch, head_dim);
+    return paged_parts(paged_plan(batch, max_pages, page_size, num_q_heads, num_kv_heads, head_dim, window, dtype, kv_split),
+                       batch, num_q_heads / num_kv_heads, head_dim).all;
 }
 
 extern "C" int cast_paged_attn_fwd(const void *q, const void *k_pages, const void *v_pages, void *out, float *lse,
@@ -775,12 +828,15 @@ extern "C" int cast_paged_attn_fwd(const void *q, const void *k_pages, const voi
     const int64_t strides[10] = {q_req, q_head, kp_page, kp_head, kp_tok, vp_page, vp_head, vp_tok, o_req, o_head};
     for (int64_t s : strides)
         if ((s * esz) % 16) return CAST_ERR_ALIGNMENT;
+    // a lane's offsets within 16 rows are 32 bits
+    if (kp_tok < 0 || vp_tok < 0 || kp_tok * esz >= 1 << 27 || vp_tok * esz >= 1 << 27) return CAST_ERR_SHAPE;
     const bool any = paged_any(page_size, max_pages);
     const PagedPlan p = paged_plan(batch, max_pages, page_size, num_q_heads, num_kv_heads, head_dim, window, dtype, kv_split);
-    if (p.items > INT32_MAX || batch > 65535) return CAST_ERR_SHAPE;
-    if (p.parts) {
+    if (!p.fits || batch > 65535 || num_q_heads > 65535) return CAST_ERR_SHAPE;
+    const PagedParts parts = paged_parts(p, batch, num_q_heads / num_kv_heads, head_dim);
+    if (parts.all) {
         if (!workspace) return CAST_ERR_NULL_POINTER;
-        if (workspace_bytes < paged_ws(p, batch, head_dim)) return CAST_ERR_WORKSPACE;
+        if (workspace_bytes < parts.all) return CAST_ERR_WORKSPACE;
         if (reinterpret_cast<uintptr_t>(workspace) & 255) return CAST_ERR_ALIGNMENT;
     }
     PagedAttnArgs a{};
@@ -805,6 +861,7 @@ extern "C" int cast_paged_attn_fwd(const void *q, const void *k_pages, const voi
     a.vp_tok = vp_tok * esz;
     a.n_pages = n_pages;
     a.page_size = page_size;
+    a.by_page = fast_div((uint32_t)page_size);
     a.batch = batch;
     a.Hq = num_q_heads;
     a.Hkv = num_kv_heads;
@@ -813,26 +870,25 @@ extern "C" int cast_paged_attn_fwd(const void *q, const void *k_pages, const voi
     a.D = head_dim;
     a.cap = max_pages * page_size;
     a.window = window;
-    a.split = p.split;
-    a.slots = p.slots;
+    a.wgs = p.wgs;
+    a.least = p.least;
+    a.prows = std::min(a.G, 16);
     a.softcap = softcap;
     a.scale = softcap > 0.f ? sm_scale : sm_scale * kPLog2e;
-    if (p.parts) {
+    if (parts.all) {
         char *ws = static_cast<char *>(workspace);
         a.head = reinterpret_cast<int32_t *>(ws);
-        ws += p_align256((size_t)batch * 2 * sizeof(int32_t));
-        a.part_ml = reinterpret_cast<float *>(ws);
-        ws += p_align256((size_t)p.items * 16 * 2 * sizeof(float));
-        a.part_o = reinterpret_cast<float *>(ws);
+        a.part_ml = reinterpret_cast<float *>(ws + parts.ml);
+        a.part_o = reinterpret_cast<float *>(ws + parts.o);
     }
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     void *args[] = {&a};
     const PagedKernel k = paged_kernel(dtype, head_dim, any);
-    if (hipLaunchKernel(k.fn, dim3((unsigned)p.items), dim3(kPWaves * 64), args, 0, st) != hipSuccess) return CAST_ERR_HIP;
-    if (p.parts) {
-        if (dtype == CAST_FP32) launch_join<PF32>(a, st);
-        else if (dtype == CAST_FP16) launch_join<PFp16>(a, st);
-        else launch_join<PBf16>(a, st);
+    if (hipLaunchKernel(k.fn, dim3((unsigned)p.wgs), dim3(kPWaves * 64), args, 0, st) != hipSuccess) return CAST_ERR_HIP;
+    if (p.least) {
+        if (dtype == CAST_FP32) launch_join<PF32>(a, k.tile, st);
+        else if (dtype == CAST_FP16) launch_join<PFp16>(a, k.tile, st);
+        else launch_join<PBf16>(a, k.tile, st);
         if (hipGetLastError() != hipSuccess) return CAST_ERR_HIP;
     }
     return CAST_OK;

@@ -81,18 +81,6 @@ struct KvSource {
 };
 enum { kSrcConcat = 0, kSrcStore = 1, kSrcPages = 2 };   // the kernels' instances by layout
 
-// Division of n in [0, 2^31) by a divisor the host knows: (mulhi(m, n) + n) >> s
-// with s = ceil(log2 d) and m = floor(2^32 * (2^s - d) / d) + 1.
-struct FastDiv {
-    uint32_t m, s;
-    __device__ __forceinline__ int div(int n) const { return (int)((__umulhi(m, (uint32_t)n) + (uint32_t)n) >> s); }
-};
-static FastDiv fast_div(uint32_t d) {
-    uint32_t s = 0;
-    while (s < 31 && (1u << s) < d) ++s;
-    return {(uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << s) - d)) / d + 1), s};
-}
-
 struct AttnArgs {
     const void *q;
     KvSource kv;
