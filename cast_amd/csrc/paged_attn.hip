@@ -51,6 +51,7 @@ namespace cast {
 constexpr float kPLn2 = 0.69314718055994530942f;
 constexpr float kPLog2e = 1.44269504088896340736f;
 constexpr int kPWaves = 4;
+constexpr int kLensLds = 1024;           // batches whose lengths a workgroup keeps in LDS for its schedule
 constexpr int kMinTiles = 2;             // fewest key tiles of a workgroup's stretch, unless the caller says
 
 struct PagedAttnArgs {
@@ -64,10 +65,11 @@ struct PagedAttnArgs {
     int32_t n_pages, page_size, batch, Hq, Hkv, G, rbs, D, cap, window;  // cap: slots a table row covers
     FastDiv by_page;    // division by page_size
     int32_t wgs;        // workgroups of the attention kernel
-    int32_t least;      // fewest tiles of a run; 0: one workgroup per unit, no runs
+    int32_t least;      // fewest tiles of a piece; 0: one workgroup per unit, no pieces
+    int32_t cut;        // pieces of exactly `least` tiles, as the caller says
     int32_t prows;      // rows of a partial: min(16, G)
     float scale, softcap;   // scale: natural scale (softcap) or times log2(e)
-    int32_t *head;      // workspace: all tiles, then each request's first tile
+    int32_t *units;     // workspace: [units][2], a unit's first partial slot and how many pieces it has (1: none, it is out)
     float *part_ml;     // [2 wgs][prows][2] running maximum (base 2) and sum; sum < 0: a page id is bad
     float *part_o;      // [2 wgs][prows][D]
 };
@@ -122,13 +124,21 @@ struct PFp16 : Fp16 {
     }
 };
 
-// ---- the schedule, found by every workgroup from the lengths.  The units
-// (request, block of 16 query heads, KV head), each a run of key tiles, lie in
-// a line, and the workgroups take equal stretches of it: with `all` tiles and
-// W workgroups, the first all % W take one tile more than the others.  A
-// workgroup walks its stretch unit by unit; a unit that it covers whole goes
-// to the output, a piece of one to a partial, of which a workgroup has at most
-// two (its first and its last).
+// ---- the schedule, found by every workgroup from the lengths.  A unit
+// (request, block of 16 query heads, KV head) is a run of key tiles.
+//  - Cut: every unit into equal pieces of at most c tiles, a workgroup each,
+//    where c is an even share of all tiles (or 9/8 of it) and the pieces are no
+//    more than the workgroups that the device holds.
+//  - Stretches, where they would be more: the units lie in a line and the
+//    workgroups take equal stretches of it (with `all` tiles and W workgroups,
+//    the first all % W take one tile more than the others).  A workgroup walks
+//    its stretch unit by unit; it meets at most two units that it does not
+//    cover whole, its first and its last.
+// A unit that a workgroup covers whole goes to the output, a piece of one to a
+// partial, two slots a workgroup.  Measured, one against the other: 8 requests
+// whose windows take 32 or 33 tiles, D = 256, cut 55.1 us, stretches 59.2 (a
+// second piece costs a join and a pipeline's start); 64 requests of 300 to 8k
+// keys cut 250 us, stretches 222 (the cut ran in one and a half rounds).
 struct PagedReq {
     int start, len, t0, tiles;   // visible slots [start, len), key tiles [t0, t0 + tiles); a tile where none is seen
 };
@@ -140,6 +150,9 @@ __device__ __forceinline__ PagedReq paged_req(const PagedAttnArgs &a, int tk, in
     r.t0 = r.start / tk;
     r.tiles = (len + tk - 1) / tk - r.t0;
     return r;
+}
+__device__ __forceinline__ int splits_of(int tiles, int c) {
+    return tiles <= c ? 1 : (int)(((uint32_t)tiles + (uint32_t)c - 1) / (uint32_t)c);
 }
 struct Stretches {
     int W, q, r;
@@ -169,50 +182,109 @@ void paged_attn_kernel(PagedAttnArgs a) {
     constexpr int VC = D / (16 * EPC);             // V chunks of a key a lane holds
     constexpr int VK = 4 * KB;                     // keys a lane holds V of
     constexpr int NA = D / 16;                     // 16-row blocks of O^T
+    constexpr bool kAhead = !(ANY && F32 && D == 256);   // two tiles in flight (here they, and 64-bit addresses, spill)
     constexpr int OP = D + 4;                      // row stride of the join's O (floats)
     __shared__ __attribute__((aligned(16))) float Os[kPWaves][16][OP];
     __shared__ float ML[kPWaves][16][2];
+    __shared__ int Lens[kLensLds];
 
     const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, l8 = lane & 7, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int dr = PAD ? a.D : D;
 
-    // ---- this workgroup's stretch [p, p_end) of tiles; lane j knows the
-    // length of request b0 + j, whose tiles start at `base` for request b
+    // ---- this workgroup's tiles [p, p_end) of the line of units, in which
+    // request b's start at `base`
     const int per = a.Hkv * a.rbs, x = blockIdx.x;
     int b0 = 0, b = 0, base = 0, p = 0, p_first = 0, p_end = 0, len_l = 0;
     if (a.least) {
-        int all = 0;
-        for (int c = 0; c < a.batch; c += 64) {
-            const int bb = c + lane;
-            const int len = bb < a.batch ? a.seq_len[bb] : 0;
-            const int n = bb < a.batch ? paged_req(a, TK, len).tiles * per : 0;
-            const int incl = p_wave_scan(n);
-            if (x == 0 && w == 0 && bb < a.batch) {
-                a.head[1 + bb] = all + incl - n;
-                if (len < 0 || len > a.cap) raise_flag(a.status, CAST_FLAG_BAD_OFFSETS);
-            }
-            all += __builtin_amdgcn_readlane(incl, 63);
-            len_l = len;
+        // (loops of little code: what runs once waits for its instructions)
+        const int *lens = a.seq_len;
+        if (a.batch <= kLensLds) {
+            for (int i = tid; i < a.batch; i += kPWaves * 64) Lens[i] = a.seq_len[i];
+            __syncthreads();
+            lens = Lens;
         }
-        if (x == 0 && tid == 0) a.head[0] = all;
-        const Stretches st(a, all);
-        if (x >= st.W) return;
-        p_first = p = st.first(x);
-        p_end = st.first(x + 1);
-        for (;; b0 += 64) {
-            if (a.batch > 64) len_l = b0 + lane < a.batch ? a.seq_len[b0 + lane] : 0;
-            const int n = b0 + lane < a.batch ? paged_req(a, TK, len_l).tiles * per : 0;
-            const int incl = p_wave_scan(n);
-            const uint64_t past = __ballot(base + incl <= p);
+        // this lane's request's tiles in the block of 64 from k on, or its
+        // units' pieces of up to c tiles
+        auto count = [&](int k, int c) __attribute__((always_inline)) {
+            len_l = lens[min(k + lane, a.batch - 1)];
+            const int n = paged_req(a, TK, len_l).tiles;
+            return k + lane >= a.batch ? 0 : (c ? splits_of(n, c) : n) * per;
+        };
+        int all = 0, c = a.cut ? a.least : 0, items = 0;
+        for (;;) {
+            int n = 0;
+#pragma unroll 1
+            for (int k = 0; k < a.batch; k += 64) n += p_wave_sum(count(k, c));
+            if (a.cut) {
+                items = n;
+                break;
+            }
+            if (c == 0) {
+                all = n;
+                c = max(a.least, (int)(((uint32_t)all + (uint32_t)a.wgs - 1) / (uint32_t)a.wgs));
+            } else if (n <= a.wgs) {
+                items = n;
+                break;
+            } else if (items || c < 8) {
+                items = c = 0;
+                break;
+            } else {
+                items = n;
+                c += c >> 3;
+            }
+        }
+        const Stretches st(a, c ? a.least : all);
+        if (x >= (c ? items : st.W)) return;
+        const int at = c ? x : st.first(x);
+#pragma unroll 1
+        for (int k = 0; k < a.batch; k += 64) {
+            const int n = count(k, c), incl = p_wave_scan(n);
+            const uint64_t past = __ballot(base + incl <= at);
+            b0 = k;
             if (~past) {
-                const int k = __builtin_ctzll(~past);
-                b = b0 + k;
-                base += __builtin_amdgcn_readlane(incl - n, k);
+                const int j = __builtin_ctzll(~past);
+                b = k + j;
+                base += __builtin_amdgcn_readlane(incl - n, j);
                 break;
             }
             base += __builtin_amdgcn_readlane(incl, 63);
         }
+        if (x == 0 && w == 0)
+            for (int k = lane; k < a.batch; k += 64)
+                if (lens[k] < 0 || lens[k] > a.cap) raise_flag(a.status, CAST_FLAG_BAD_OFFSETS);
+        if (c) {
+            const int tiles = paged_req(a, TK, __builtin_amdgcn_readlane(len_l, b - b0)).tiles, ns = splits_of(tiles, c);
+            const int unit = (int)((uint32_t)(x - base) / (uint32_t)ns), s = x - base - unit * ns;
+            if (s == 0 && tid == 0) {
+                a.units[2 * (b * per + unit)] = 2 * x;
+                a.units[2 * (b * per + unit) + 1] = ns;
+            }
+            base = 0;
+            p = unit * tiles + (int)((int64_t)tiles * s / ns);
+            p_end = unit * tiles + (int)((int64_t)tiles * (s + 1) / ns);
+        } else {
+            p = at;
+            p_end = st.first(x + 1);
+            // the units that begin in the stretch: a lane each
+            if (w == 0) {
+                int bb = b, from = base;
+                for (int left = p; left < p_end;) {
+                    const int tiles = paged_req(a, TK, lens[bb]).tiles;
+                    for (int u = lane; u < per; u += 64) {
+                        const int first = from + u * tiles;
+                        if (first >= p && first < p_end) {
+                            a.units[2 * (bb * per + u)] = 2 * x + (first != p);
+                            a.units[2 * (bb * per + u) + 1] = st.of(first + tiles - 1) - x + 1;
+                        }
+                    }
+                    from += tiles * per;
+                    left = from;
+                    ++bb;
+                }
+            }
+        }
+        p_first = p;
     } else {
         b = (int)((uint32_t)x / (uint32_t)per);
         b0 = b;
@@ -222,56 +294,62 @@ void paged_attn_kernel(PagedAttnArgs a) {
         p_end = p + tiles;
         if (x == b * per && tid == 0 && (len_l < 0 || len_l > a.cap)) raise_flag(a.status, CAST_FLAG_BAD_OFFSETS);
     }
-    for (;;) {
-    // (wave-uniform all along; told so, that addresses stay scalar)
-    p = __builtin_amdgcn_readfirstlane(p);
-    p_end = __builtin_amdgcn_readfirstlane(p_end);
-    base = __builtin_amdgcn_readfirstlane(base);
-    b = __builtin_amdgcn_readfirstlane(b);
-    b0 = __builtin_amdgcn_readfirstlane(b0);
-    const PagedReq rq = paged_req(a, TK, __builtin_amdgcn_readlane(len_l, b - b0));
-    const int unit = (int)((uint32_t)(p - base) / (uint32_t)rq.tiles), ta = p - base - unit * rq.tiles;
-    const int nt = min(p_end - p, rq.tiles - ta);  // tiles of this piece
-    const bool whole = nt == rq.tiles;
-    const int rb = unit / a.Hkv, h = unit - rb * a.Hkv;
-    const int key0 = (rq.t0 + ta) * TK + w * WK;   // the wave's first key
-    const int rows = min(16, a.G - rb * 16);       // query heads of this block
-    const int hq = h * a.G + rb * 16 + l16;
+    // (wave-uniform all along; told so, that branches and addresses are scalar)
+    auto uni = [](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(v); };
+    p = uni(p), p_first = uni(p_first), p_end = uni(p_end), base = uni(base), b = uni(b), b0 = uni(b0);
+    // lane j of a wave knows the length of request b0 + j
+    auto lengths = [&](int from) __attribute__((always_inline)) {
+        b0 = from;
+        len_l = a.seq_len[min(from + lane, a.batch - 1)];
+    };
+    // The piece of the line at tile p, which lies in request b, whose tiles
+    // start at `base`.
+    struct Piece {
+        int b, h, rb, start, len;   // visible slots [start, len)
+        int key0, nt;               // the wave's first key, tiles
+        bool whole;                 // all of its unit
+    };
+    auto piece = [&](int p, int b, int base) __attribute__((always_inline)) {
+        const PagedReq rq = paged_req(a, TK, __builtin_amdgcn_readlane(len_l, b - b0));
+        const int unit = (int)((uint32_t)(p - base) / (uint32_t)rq.tiles), ta = p - base - unit * rq.tiles;
+        Piece c;
+        c.b = b;
+        c.rb = unit / a.Hkv;
+        c.h = unit - c.rb * a.Hkv;
+        c.start = rq.start;
+        c.len = rq.len;
+        c.key0 = (rq.t0 + ta) * TK + w * WK;
+        c.nt = min(p_end - p, rq.tiles - ta);
+        c.whole = c.nt == rq.tiles;
+        return c;
+    };
 
-    // ---- Q^T: head l16 of the block, chunks as K's
+    // ---- Q^T: head l16 of the piece's block, chunks as K's
     uint32_t qraw[KC][4];
-    {
-        const T *qp = static_cast<const T *>(a.q) + (int64_t)b * a.q_req + (int64_t)hq * a.q_head;
+    auto load_q = [&](const Piece &c) __attribute__((always_inline)) {
+        const T *qp = static_cast<const T *>(a.q) + (int64_t)c.b * a.q_req + (int64_t)(c.h * a.G + c.rb * 16 + l16) * a.q_head;
 #pragma unroll
-        for (int c = 0; c < KC; ++c) {
-            const int d = F32 ? c * 16 + g * 4 : c * 32 + g * 8;
-            const bool in = l16 < rows && (!PAD || d < dr);
-            const u32x4 x = in ? *reinterpret_cast<const u32x4 *>(qp + d) : u32x4{};
+        for (int k = 0; k < KC; ++k) {
+            const int d = F32 ? k * 16 + g * 4 : k * 32 + g * 8;
+            const bool in = l16 < a.G - c.rb * 16 && (!PAD || d < dr);
+            const u32x4 y = in ? *reinterpret_cast<const u32x4 *>(qp + d) : u32x4{};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) qraw[c][i] = x[i];
+            for (int i = 0; i < 4; ++i) qraw[k][i] = y[i];
         }
-    }
-    floatx4 acc[NA];
-#pragma unroll
-    for (int i = 0; i < NA; ++i) acc[i] = floatx4{};
-    float m = -INFINITY, l = 0.f;
-    bool bad = false, again = false;
+    };
 
     // ---- page ids.  Without ANY a 16-key block lies within one page: lane
     // 2 i + t (KB = 2) or i (KB = 1) holds the id of block t of tile i0 + i.
-    const char *kbase = static_cast<const char *>(a.k) + (int64_t)h * a.kp_head;
-    const char *vbase = static_cast<const char *>(a.v) + (int64_t)h * a.vp_head;
-    const int32_t *row = a.table + (int64_t)b * a.table_ld;
-    auto seen = [&](int key) __attribute__((always_inline)) { return min(max(key, rq.start), rq.len - 1); };
-    auto page_id = [&](int key) __attribute__((always_inline)) {   // of a visible key; always a page of the pool
-        const int id = row[a.by_page.div(key)];
+    auto seen = [&](const Piece &c, int key) __attribute__((always_inline)) { return min(max(key, c.start), c.len - 1); };
+    auto page_id = [&](const Piece &c, int key, bool &bad) __attribute__((always_inline)) {   // of a visible key; always a page of the pool
+        const int id = a.table[(int64_t)c.b * a.table_ld + a.by_page.div(key)];
         bad |= id < 0 || id >= a.n_pages;
         return min(max(id, 0), a.n_pages - 1);
     };
-    int ids = 0;
-    auto load_ids = [&](int i0) __attribute__((always_inline)) {
-        const int i = min(i0 + lane / KB, nt - 1);
-        ids = page_id(seen(key0 + i * TK + (lane % KB) * 16));
+    auto load_ids = [&](const Piece &c, int i0, bool &bad) __attribute__((always_inline)) {
+        if (ANY || c.len == 0) return 0;
+        const int i = min(i0 + lane / KB, c.nt - 1);
+        return page_id(c, seen(c, c.key0 + i * TK + (lane % KB) * 16), bad);
     };
 
     struct Tile {
@@ -291,23 +369,28 @@ void paged_attn_kernel(PagedAttnArgs a) {
         const int d = (c * 16 + l16) * EPC;
         return PAD && d >= dr ? kNowhere : (uint32_t)(4 * g + r) * (uint32_t)a.vp_tok + (uint32_t)(d * E::kBytes);
     };
-    auto block = [&](const char *base, int keys, int64_t tok) __attribute__((always_inline)) {
+    auto block = [&](const char *from, int keys, int64_t tok) __attribute__((always_inline)) {
         const int bytes = keys > 0 ? (min(keys, 16) - 1) * (int)tok + dr * E::kBytes : 0;
-        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, bytes, 0x00020000);
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(from), 0, bytes, 0x00020000);
     };
     auto set_v = [&](Tile &t, int j, int c, auto y) __attribute__((always_inline)) {
 #pragma unroll
         for (int e = 0; e < VW; ++e) t.v[j][c][e] = y[e];
     };
-    auto load_tile = [&](Tile &t, int i) __attribute__((always_inline)) {
-        const int kt = key0 + i * TK;
+    // tile i of the piece (its ids in `ids`, unless ANY)
+    auto load_tile = [&](Tile &t, const Piece &cur, int i, int ids, bool &bad) __attribute__((always_inline)) {
+        if (ANY && (cur.len == 0 || i >= cur.nt)) return;
+        const char *kbase = static_cast<const char *>(a.k) + (int64_t)cur.h * a.kp_head;
+        const char *vbase = static_cast<const char *>(a.v) + (int64_t)cur.h * a.vp_head;
+        const int kt = cur.key0 + i * TK;
 #pragma unroll
         for (int t16 = 0; t16 < KB; ++t16) {
             const int kb = kt + 16 * t16;
             if constexpr (!ANY) {
                 // the block's seen keys share a page
-                const int kc = seen(kb), off = kb - a.by_page.div(kc) * a.page_size;
-                const int keys = kb + 16 > rq.start ? rq.len - kb : 0;
+                // (no branch: a tile past the piece's last is a load of nothing)
+                const int kc = max(seen(cur, kb), 0), off = kb - a.by_page.div(kc) * a.page_size;
+                const int keys = i < cur.nt && kb + 16 > cur.start ? cur.len - kb : 0;
                 const int64_t id = __builtin_amdgcn_readlane(ids, (i % (64 / KB)) * KB + t16);
                 const __amdgpu_buffer_rsrc_t kr = block(kbase + id * a.kp_page + off * a.kp_tok, keys, a.kp_tok);
                 const __amdgpu_buffer_rsrc_t vr = block(vbase + id * a.vp_page + off * a.vp_tok, keys, a.vp_tok);
@@ -325,8 +408,8 @@ void paged_attn_kernel(PagedAttnArgs a) {
                     }
             } else {
                 // every key's own page; keys that are not seen are clamped into those that are
-                const int key = seen(kb + l16);
-                const int id = page_id(key), off = key - a.by_page.div(key) * a.page_size;
+                const int key = seen(cur, kb + l16);
+                const int id = page_id(cur, key, bad), off = key - a.by_page.div(key) * a.page_size;
                 auto row_at = [&](const char *pool, int64_t page, int64_t tok, int from) __attribute__((always_inline)) {
                     return pool + (int64_t)__shfl(id, from) * page + (int64_t)__shfl(off, from) * tok;
                 };
@@ -336,8 +419,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
 #pragma unroll
                     for (int c = y; c < KC; c += 2) {
                         const int d = ((c >> 1) * 8 + (l16 >> 3) * 4 + g) * KE;
-                        const u32x4 z = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(kp + min(d, dr - KE) * E::kBytes));
-                        t.k[t16][c] = d < dr ? z : u32x4{};
+                        t.k[t16][c] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(kp + min(d, dr - KE) * E::kBytes));
                     }
                 }
 #pragma unroll
@@ -357,9 +439,12 @@ void paged_attn_kernel(PagedAttnArgs a) {
     };
 
     const float inv_cap = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
-    auto use_tile = [&](Tile &t, int i) __attribute__((always_inline)) {
-        const int kt = key0 + i * TK;
-        const bool edge = kt < rq.start || kt + WK > rq.len;
+    floatx4 acc[NA];
+    float m, l;
+    bool again;   // see below
+    auto use_tile = [&](Tile &t, const Piece &cur, int i) __attribute__((always_inline)) {
+        const int kt = cur.key0 + i * TK;
+        const bool edge = kt < cur.start || kt + WK > cur.len;
         float p[KB][4];
         __builtin_amdgcn_sched_barrier(0);   // (in this order: a tile's registers, not two stages')
         // ---- scores, base 2
@@ -376,6 +461,10 @@ void paged_attn_kernel(PagedAttnArgs a) {
                     const uint32_t near = t.k[t16][c & ~1][e], far = t.k[t16][c | 1][e];
                     kx[e] = c & 1 ? (uint32_t)__builtin_amdgcn_update_dpp((int)far, (int)near, 0x128, 0xf, 0x3, false)
                                   : (uint32_t)__builtin_amdgcn_update_dpp((int)near, (int)far, 0x128, 0xf, 0xc, false);
+                }
+                if constexpr (ANY) {
+                    // (chunks past the head dim were read from its last one)
+                    if ((F32 ? c * 16 + g * 4 : c * 32 + g * 8) >= dr) kx = u32x4{};
                 }
                 if constexpr (F32) {
 #pragma unroll
@@ -411,10 +500,10 @@ void paged_attn_kernel(PagedAttnArgs a) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int key = kt + 16 * t16 + 4 * g + r;
-                    if (key < rq.start || key >= rq.len) {
+                    if (key < cur.start || key >= cur.len) {
                         p[t16][r] = -INFINITY;
                         // (rows past the last key were loaded as zeros)
-                        if (ANY || key < rq.start) {
+                        if (ANY || key < cur.start) {
 #pragma unroll
                             for (int c = 0; c < VC; ++c)
 #pragma unroll
@@ -496,19 +585,52 @@ void paged_attn_kernel(PagedAttnArgs a) {
 
     // where the wave's O^T lies in its part of the join's LDS
     auto place = [&](int c, int r) __attribute__((always_inline)) { return &Os[w][l16][(c * 16 + 4 * g + r) * EPC]; };
-    if (rq.len > 0) {
+    // ---- piece by piece: the next one's page ids are loaded when one begins,
+    // its first tile and Q before the one's join, whose LDS round trip they
+    // run beside
+    Tile even;
+    bool bad = false;
+    Piece cur = piece(p, b, base);
+    int ids = load_ids(cur, 0, bad);
+    load_q(cur);
+    if (!ANY) load_tile(even, cur, 0, ids, bad);
+    for (;;) {
+    if (ANY) load_tile(even, cur, 0, ids, bad);
+    const int p_next = uni(p + cur.nt);
+    const bool more = p_next < p_end;
+    bool bad_next = false;
+    int ids_next = 0;
+    if (more) {
+        const int after = base + paged_req(a, TK, __builtin_amdgcn_readlane(len_l, b - b0)).tiles * per;
+        if (p_next == after) {
+            base = after;
+            if (++b == b0 + 64) lengths(b);
+        }
+        ids_next = load_ids(piece(p_next, b, base), 0, bad_next);
+    }
+#pragma unroll
+    for (int n = 0; n < NA; ++n) acc[n] = floatx4{};
+    m = -INFINITY;
+    l = 0.f;
+    again = false;
+    const int rows = min(16, a.G - cur.rb * 16);   // query heads of this block
+    if (cur.len > 0) {
         for (;;) {
-            Tile buf[2];
-            if constexpr (!ANY) load_ids(0);
-            load_tile(buf[0], 0);
-            for (int i = 0; i < nt; i += 2) {
-                if (i + 1 < nt) load_tile(buf[1], i + 1);
-                use_tile(buf[0], i);
-                if (i + 1 >= nt) break;
-                if constexpr (!ANY)
-                    if ((i + 2) % (64 / KB) == 0) load_ids(i + 2);
-                if (i + 2 < nt) load_tile(buf[0], i + 2);
-                use_tile(buf[1], i + 1);
+            if constexpr (!kAhead) {
+                for (int i = 0;;) {
+                    use_tile(even, cur, i);
+                    if (++i >= cur.nt) break;
+                    load_tile(even, cur, i, ids, bad);
+                }
+            }
+            for (int i = kAhead ? 0 : cur.nt; i < cur.nt; i += 2) {
+                Tile odd;
+                load_tile(odd, cur, i + 1, ids, bad);
+                use_tile(even, cur, i);
+                if (i + 1 >= cur.nt) break;
+                if (!ANY && (i + 2) % (64 / KB) == 0) ids = load_ids(cur, i + 2, bad);
+                load_tile(even, cur, i + 2, ids, bad);
+                use_tile(odd, cur, i + 1);
             }
             if (F32 || again) break;
             // An infinite V times a weight's second term, of either sign or
@@ -533,12 +655,22 @@ void paged_attn_kernel(PagedAttnArgs a) {
             m = -INFINITY;
             l = 0.f;
             again = true;
+            ids = load_ids(cur, 0, bad);
+            load_tile(even, cur, 0, ids, bad);
         }
+    }
+    const Piece done = cur;
+    const bool wbad = __any(bad);
+    if (more) {
+        cur = piece(p_next, b, base);
+        ids = ids_next;
+        bad = bad_next;
+        load_q(cur);
+        if (!ANY) load_tile(even, cur, 0, ids, bad);
     }
 
     // ---- join the four waves
     l = quad_sum(l);
-    const bool wbad = __any(bad);
     if (l16 < rows) {
 #pragma unroll
         for (int c = 0; c < VC; ++c)
@@ -574,8 +706,8 @@ void paged_attn_kernel(PagedAttnArgs a) {
             for (int e = 0; e < 4; ++e) o[e] = fmaf(y[e], f, o[e]);
         }
         if (rejected && u == 0) raise_flag(a.status, CAST_FLAG_BAD_PAGE);
-        const int head = h * a.G + rb * 16 + q;
-        if (!whole) {
+        const int head = done.h * a.G + done.rb * 16 + q;
+        if (!done.whole) {
             const int64_t at = (int64_t)(2 * x + (p != p_first)) * a.prows + q;
             *reinterpret_cast<floatx4 *>(a.part_o + at * dr + d) = o;
             if (d == 0) {
@@ -584,7 +716,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
             }
         } else {
             const float inv = rejected || lt == 0.f ? 0.f : 1.f / (lt * E::kPScale);
-            T *op = static_cast<T *>(a.out) + (int64_t)b * a.o_req + (int64_t)head * a.o_head + d;
+            T *op = static_cast<T *>(a.out) + (int64_t)done.b * a.o_req + (int64_t)head * a.o_head + d;
             if (rejected || lt == 0.f) o = floatx4{};
             if constexpr (F32) {
                 *reinterpret_cast<floatx4 *>(op) = o * inv;
@@ -593,19 +725,11 @@ void paged_attn_kernel(PagedAttnArgs a) {
                 *reinterpret_cast<u32x2 *>(op) = y;
             }
             if (d == 0 && a.lse)
-                a.lse[(int64_t)b * a.Hq + head] = rejected || lt == 0.f ? -INFINITY : (ms + log2f(lt)) * kPLn2;
+                a.lse[(int64_t)done.b * a.Hq + head] = rejected || lt == 0.f ? -INFINITY : (ms + log2f(lt)) * kPLn2;
         }
     }
-    // ---- the next piece
-    p += nt;
-    if (p >= p_end) return;
-    if (p == base + rq.tiles * per) {
-        base = p;
-        if (++b == b0 + 64) {
-            b0 = b;
-            len_l = b0 + lane < a.batch ? a.seq_len[b0 + lane] : 0;
-        }
-    }
+    if (!more) return;
+    p = p_next;
     __syncthreads();   // (the join's LDS is read)
     }
 }
@@ -614,21 +738,18 @@ void paged_attn_kernel(PagedAttnArgs a) {
 // float4 of the head dim a lane, walk every NG-th split with up to four in
 // flight and their own running maximum, then join through LDS.
 template <typename E, int LP>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int tk) {
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
     using T = typename E::T;
     constexpr int NG = 256 / LP;
     __shared__ __attribute__((aligned(16))) floatx4 Os[NG][LP];
     __shared__ float ML[NG][2];
     const int b = blockIdx.y, head = blockIdx.x;
-    const PagedReq rq = paged_req(a, tk, a.seq_len[b]);
     const int h = head / a.G, in = head - h * a.G, rb = in / 16, q = in - rb * 16;
-    const Stretches st(a, a.head[0]);
-    const int first = a.head[1 + b] + (rb * a.Hkv + h) * rq.tiles;
-    const int x0 = st.of(first), ns = st.of(first + rq.tiles - 1) - x0 + 1;
+    const int32_t *unit = a.units + 2 * (((int64_t)b * a.rbs + rb) * a.Hkv + h);
+    const int slot = unit[0], ns = unit[1];
     if (ns <= 1) return;
-    // the first piece is its workgroup's last one, unless the unit starts there
-    const int late = st.first(x0) != first;
-    auto row_of = [&](int s) __attribute__((always_inline)) { return (int64_t)(2 * (x0 + s) + (s == 0 ? late : 0)) * a.prows + q; };
+    // the pieces after the first are their workgroups' first ones
+    auto row_of = [&](int s) __attribute__((always_inline)) { return (int64_t)(s ? (slot & ~1) + 2 * s : slot) * a.prows + q; };
     const int grp = threadIdx.x / LP, d = (threadIdx.x % LP) * 4, dl = min(d, a.D - 4);
     float m = -INFINITY, l = 0.f;
     bool rejected = false;
@@ -695,11 +816,11 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int tk
     if (d == 0 && a.lse) a.lse[(int64_t)b * a.Hq + head] = none ? -INFINITY : (ms + log2f(l)) * kPLn2;
 }
 template <typename E>
-static void launch_join(const PagedAttnArgs &a, int tk, hipStream_t st) {
+static void launch_join(const PagedAttnArgs &a, hipStream_t st) {
     const dim3 grid((unsigned)a.Hq, (unsigned)a.batch);
-    if (a.D <= 64) paged_join_kernel<E, 16><<<grid, 256, 0, st>>>(a, tk);
-    else if (a.D <= 128) paged_join_kernel<E, 32><<<grid, 256, 0, st>>>(a, tk);
-    else paged_join_kernel<E, 64><<<grid, 256, 0, st>>>(a, tk);
+    if (a.D <= 64) paged_join_kernel<E, 16><<<grid, 256, 0, st>>>(a);
+    else if (a.D <= 128) paged_join_kernel<E, 32><<<grid, 256, 0, st>>>(a);
+    else paged_join_kernel<E, 64><<<grid, 256, 0, st>>>(a);
 }
 
 // --------------------------------------------------------------------------
@@ -759,7 +880,7 @@ static int paged_slots(const PagedKernel &k) {
 }
 
 struct PagedPlan {
-    int32_t wgs, least;   // as PagedAttnArgs
+    int32_t wgs, least, cut;   // as PagedAttnArgs
     bool fits;            // tile indices fit 31 bits for any lengths
 };
 static PagedPlan paged_plan(int32_t batch, int32_t max_pages, int32_t page_size, int32_t Hq, int32_t Hkv, int32_t D,
@@ -770,20 +891,20 @@ static PagedPlan paged_plan(int32_t batch, int32_t max_pages, int32_t page_size,
     if (window > 0 && window < keys) keys = (int64_t)window + k.tile - 1;   // (a window may start inside a tile)
     const int64_t tiles = (keys + k.tile - 1) / k.tile;
     const int64_t least = kv_split > 0 ? ((int64_t)kv_split + k.tile - 1) / k.tile : kMinTiles;
-    if (kv_split < 0 || tiles <= least) return {units > INT_MAX ? 0 : (int32_t)units, 0, units <= INT_MAX};
-    if (units > INT_MAX / tiles) return {0, 0, false};
-    const int64_t most = (units * tiles + least - 1) / least;
+    if (kv_split < 0 || tiles <= least) return {units > INT_MAX ? 0 : (int32_t)units, 0, 0, units <= INT_MAX};
+    if (units > INT_MAX / tiles) return {0, 0, 0, false};
+    const int64_t most = units * ((tiles + least - 1) / least);
     const int64_t wgs = kv_split > 0 ? most : std::min<int64_t>(most, paged_slots(k));
-    return {(int32_t)wgs, (int32_t)least, true};
+    return {(int32_t)wgs, (int32_t)least, kv_split > 0, true};
 }
 static size_t p_align256(size_t x) { return (x + 255) & ~(size_t)255; }
 struct PagedParts {
     size_t ml, o, all;   // offsets of the partials' sums and outputs, bytes in all
 };
-static PagedParts paged_parts(const PagedPlan &p, int32_t batch, int32_t G, int32_t D) {
+static PagedParts paged_parts(const PagedPlan &p, int32_t batch, int32_t Hkv, int32_t G, int32_t D) {
     const size_t rows = (size_t)2 * p.wgs * std::min(G, 16);
     PagedParts s{};
-    s.ml = p_align256(((size_t)batch + 1) * sizeof(int32_t));
+    s.ml = p_align256((size_t)batch * Hkv * ((G + 15) / 16) * 2 * sizeof(int32_t));
     s.o = s.ml + p_align256(rows * 2 * sizeof(float));
     s.all = p.least ? s.o + p_align256(rows * D * sizeof(float)) : 0;
     return s;
@@ -801,7 +922,7 @@ extern "C" size_t cast_paged_attn_workspace_size(int32_t batch, int32_t max_page
         return 0;
     if (dtype != CAST_BF16 && dtype != CAST_FP16 && dtype != CAST_FP32) return 0;
     return paged_parts(paged_plan(batch, max_pages, page_size, num_q_heads, num_kv_heads, head_dim, window, dtype, kv_split),
-                       batch, num_q_heads / num_kv_heads, head_dim).all;
+                       batch, num_kv_heads, num_q_heads / num_kv_heads, head_dim).all;
 }
 
 extern "C" int cast_paged_attn_fwd(const void *q, const void *k_pages, const void *v_pages, void *out, float *lse,
@@ -833,7 +954,7 @@ extern "C" int cast_paged_attn_fwd(const void *q, const void *k_pages, const voi
     const bool any = paged_any(page_size, max_pages);
     const PagedPlan p = paged_plan(batch, max_pages, page_size, num_q_heads, num_kv_heads, head_dim, window, dtype, kv_split);
     if (!p.fits || batch > 65535 || num_q_heads > 65535) return CAST_ERR_SHAPE;
-    const PagedParts parts = paged_parts(p, batch, num_q_heads / num_kv_heads, head_dim);
+    const PagedParts parts = paged_parts(p, batch, num_kv_heads, num_q_heads / num_kv_heads, head_dim);
     if (parts.all) {
         if (!workspace) return CAST_ERR_NULL_POINTER;
         if (workspace_bytes < parts.all) return CAST_ERR_WORKSPACE;
@@ -872,12 +993,13 @@ extern "C" int cast_paged_attn_fwd(const void *q, const void *k_pages, const voi
     a.window = window;
     a.wgs = p.wgs;
     a.least = p.least;
+    a.cut = p.cut;
     a.prows = std::min(a.G, 16);
     a.softcap = softcap;
     a.scale = softcap > 0.f ? sm_scale : sm_scale * kPLog2e;
     if (parts.all) {
         char *ws = static_cast<char *>(workspace);
-        a.head = reinterpret_cast<int32_t *>(ws);
+        a.units = reinterpret_cast<int32_t *>(ws);
         a.part_ml = reinterpret_cast<float *>(ws + parts.ml);
         a.part_o = reinterpret_cast<float *>(ws + parts.o);
     }
@@ -886,9 +1008,9 @@ extern "C" int cast_paged_attn_fwd(const void *q, const void *k_pages, const voi
     const PagedKernel k = paged_kernel(dtype, head_dim, any);
     if (hipLaunchKernel(k.fn, dim3((unsigned)p.wgs), dim3(kPWaves * 64), args, 0, st) != hipSuccess) return CAST_ERR_HIP;
     if (p.least) {
-        if (dtype == CAST_FP32) launch_join<PF32>(a, k.tile, st);
-        else if (dtype == CAST_FP16) launch_join<PFp16>(a, k.tile, st);
-        else launch_join<PBf16>(a, k.tile, st);
+        if (dtype == CAST_FP32) launch_join<PF32>(a, st);
+        else if (dtype == CAST_FP16) launch_join<PFp16>(a, st);
+        else launch_join<PBf16>(a, st);
         if (hipGetLastError() != hipSuccess) return CAST_ERR_HIP;
     }
     return CAST_OK;
