@@ -51,6 +51,10 @@ namespace cast {
 constexpr float kPLn2 = 0.69314718055994530942f;
 constexpr float kPLog2e = 1.44269504088896340736f;
 constexpr int kPWaves = 4;
+// What a piece costs beside its tiles, in tiles of 32 KB (head dim 64) and of
+// 64 KB and more: 200 requests of up to 1k keys at D = 64, fp16, 43.3, 36.5, 35.2
+// and 35.9 us for 0 to 3; 64 of 300 to 8k at D = 128, bf16, 219.5, 222, 225, 230.
+constexpr int piece_cost(int D) { return D == 64 ? 2 : 1; }
 constexpr int kLensLds = 1024;           // batches whose lengths a workgroup keeps in LDS for its schedule
 constexpr int kMinTiles = 2;             // fewest key tiles of a workgroup's stretch, unless the caller says
 
@@ -129,11 +133,12 @@ struct PFp16 : Fp16 {
 //  - Cut: every unit into equal pieces of at most c tiles, a workgroup each,
 //    where c is an even share of all tiles (or 9/8 of it) and the pieces are no
 //    more than the workgroups that the device holds.
-//  - Stretches, where they would be more: the units lie in a line and the
-//    workgroups take equal stretches of it (with `all` tiles and W workgroups,
-//    the first all % W take one tile more than the others).  A workgroup walks
-//    its stretch unit by unit; it meets at most two units that it does not
-//    cover whole, its first and its last.
+//  - Stretches, where they would be more: the units lie in a line, piece_cost
+//    empty places (what a piece costs beside its tiles) and then a place per
+//    tile each, and the workgroups take equal stretches of it (with `all`
+//    places and W workgroups, the first all % W take one more than the others).
+//    A workgroup walks its stretch unit by unit; it meets at most two units
+//    that it does not cover whole, its first and its last.
 // A unit that a workgroup covers whole goes to the output, a piece of one to a
 // partial, two slots a workgroup.  Measured, one against the other: 8 requests
 // whose windows take 32 or 33 tiles, D = 256, cut 55.1 us, stretches 59.2 (a
@@ -161,10 +166,10 @@ struct Stretches {
         q = (int)((uint32_t)all / (uint32_t)W);
         r = all - q * W;
     }
-    __device__ __forceinline__ int first(int x) const { return x * q + min(x, r); }   // workgroup x's first tile
-    __device__ __forceinline__ int of(int tile) const {                               // whose tile it is
+    __device__ __forceinline__ int first(int x) const { return x * q + min(x, r); }   // workgroup x's first place
+    __device__ __forceinline__ int of(int at) const {                                 // whose place it is
         const int wide = r * (q + 1);
-        return tile < wide ? (int)((uint32_t)tile / (uint32_t)(q + 1)) : r + (int)((uint32_t)(tile - wide) / (uint32_t)q);
+        return at < wide ? (int)((uint32_t)at / (uint32_t)(q + 1)) : r + (int)((uint32_t)(at - wide) / (uint32_t)q);
     }
 };
 
@@ -192,10 +197,10 @@ void paged_attn_kernel(PagedAttnArgs a) {
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int dr = PAD ? a.D : D;
 
-    // ---- this workgroup's tiles [p, p_end) of the line of units, in which
-    // request b's start at `base`
+    // ---- this workgroup's places [p, p_end) of the line of units, in which
+    // request b's start at `base`; a unit is `cost` empty places and its tiles
     const int per = a.Hkv * a.rbs, x = blockIdx.x;
-    int b0 = 0, b = 0, base = 0, p = 0, p_first = 0, p_end = 0, len_l = 0;
+    int b0 = 0, b = 0, base = 0, p = 0, p_first = 0, p_end = 0, len_l = 0, cost = 0;
     if (a.least) {
         // (loops of little code: what runs once waits for its instructions)
         const int *lens = a.seq_len;
@@ -204,12 +209,12 @@ void paged_attn_kernel(PagedAttnArgs a) {
             __syncthreads();
             lens = Lens;
         }
-        // this lane's request's tiles in the block of 64 from k on, or its
-        // units' pieces of up to c tiles
+        // the places of this lane's request in the block of 64 from k on, or
+        // its units' pieces of up to c tiles
         auto count = [&](int k, int c) __attribute__((always_inline)) {
             len_l = lens[min(k + lane, a.batch - 1)];
             const int n = paged_req(a, TK, len_l).tiles;
-            return k + lane >= a.batch ? 0 : (c ? splits_of(n, c) : n) * per;
+            return k + lane >= a.batch ? 0 : (c ? splits_of(n, c) : n + piece_cost(D)) * per;
         };
         int all = 0, c = a.cut ? a.least : 0, items = 0;
         for (;;) {
@@ -222,7 +227,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
             }
             if (c == 0) {
                 all = n;
-                c = max(a.least, (int)(((uint32_t)all + (uint32_t)a.wgs - 1) / (uint32_t)a.wgs));
+                c = max(a.least, (int)(((uint32_t)(all - a.batch * per * piece_cost(D)) + (uint32_t)a.wgs - 1) / (uint32_t)a.wgs));
             } else if (n <= a.wgs) {
                 items = n;
                 break;
@@ -264,25 +269,30 @@ void paged_attn_kernel(PagedAttnArgs a) {
             p = unit * tiles + (int)((int64_t)tiles * s / ns);
             p_end = unit * tiles + (int)((int64_t)tiles * (s + 1) / ns);
         } else {
+            cost = piece_cost(D);
             p = at;
             p_end = st.first(x + 1);
-            // the units that begin in the stretch: a lane each
+            // the units whose first tile lies in the stretch: a lane each
             if (w == 0) {
                 int bb = b, from = base;
-                for (int left = p; left < p_end;) {
+                for (int left = p; left < p_end; ++bb) {
                     const int tiles = paged_req(a, TK, lens[bb]).tiles;
                     for (int u = lane; u < per; u += 64) {
-                        const int first = from + u * tiles;
+                        const int unit = from + u * (tiles + cost), first = unit + cost;
                         if (first >= p && first < p_end) {
-                            a.units[2 * (bb * per + u)] = 2 * x + (first != p);
+                            // (a stretch that starts in front of the unit has a piece of the one before)
+                            a.units[2 * (bb * per + u)] = 2 * x + (p < unit);
                             a.units[2 * (bb * per + u) + 1] = st.of(first + tiles - 1) - x + 1;
                         }
                     }
-                    from += tiles * per;
-                    left = from;
-                    ++bb;
+                    left = from += (tiles + cost) * per;
                 }
             }
+            // on to its first tile
+            const int width = paged_req(a, TK, __builtin_amdgcn_readlane(len_l, b - b0)).tiles + cost;
+            const int in = (int)((uint32_t)(p - base) % (uint32_t)width);
+            if (in < cost) p += cost - in;
+            if (p >= p_end) return;
         }
         p_first = p;
     } else {
@@ -302,16 +312,17 @@ void paged_attn_kernel(PagedAttnArgs a) {
         b0 = from;
         len_l = a.seq_len[min(from + lane, a.batch - 1)];
     };
-    // The piece of the line at tile p, which lies in request b, whose tiles
-    // start at `base`.
+    // The piece of the line at place p, a tile of request b, whose places start
+    // at `base`.
     struct Piece {
         int b, h, rb, start, len;   // visible slots [start, len)
         int key0, nt;               // the wave's first key, tiles
-        bool whole;                 // all of its unit
+        bool whole, last;           // all of its unit, up to its end
     };
     auto piece = [&](int p, int b, int base) __attribute__((always_inline)) {
         const PagedReq rq = paged_req(a, TK, __builtin_amdgcn_readlane(len_l, b - b0));
-        const int unit = (int)((uint32_t)(p - base) / (uint32_t)rq.tiles), ta = p - base - unit * rq.tiles;
+        const int width = rq.tiles + cost, unit = (int)((uint32_t)(p - base) / (uint32_t)width);
+        const int ta = p - base - unit * width - cost;
         Piece c;
         c.b = b;
         c.rb = unit / a.Hkv;
@@ -321,6 +332,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
         c.key0 = (rq.t0 + ta) * TK + w * WK;
         c.nt = min(p_end - p, rq.tiles - ta);
         c.whole = c.nt == rq.tiles;
+        c.last = c.nt == rq.tiles - ta;
         return c;
     };
 
@@ -596,13 +608,13 @@ void paged_attn_kernel(PagedAttnArgs a) {
     if (!ANY) load_tile(even, cur, 0, ids, bad);
     for (;;) {
     if (ANY) load_tile(even, cur, 0, ids, bad);
-    const int p_next = uni(p + cur.nt);
+    const int p_next = uni(p + cur.nt + (cur.last ? cost : 0));
     const bool more = p_next < p_end;
     bool bad_next = false;
     int ids_next = 0;
     if (more) {
-        const int after = base + paged_req(a, TK, __builtin_amdgcn_readlane(len_l, b - b0)).tiles * per;
-        if (p_next == after) {
+        const int after = base + (paged_req(a, TK, __builtin_amdgcn_readlane(len_l, b - b0)).tiles + cost) * per;
+        if (p_next >= after) {
             base = after;
             if (++b == b0 + 64) lengths(b);
         }
@@ -892,7 +904,7 @@ static PagedPlan paged_plan(int32_t batch, int32_t max_pages, int32_t page_size,
     const int64_t tiles = (keys + k.tile - 1) / k.tile;
     const int64_t least = kv_split > 0 ? ((int64_t)kv_split + k.tile - 1) / k.tile : kMinTiles;
     if (kv_split < 0 || tiles <= least) return {units > INT_MAX ? 0 : (int32_t)units, 0, 0, units <= INT_MAX};
-    if (units > INT_MAX / tiles) return {0, 0, 0, false};
+    if (units > INT_MAX / (tiles + piece_cost(64))) return {0, 0, 0, false};
     const int64_t most = units * ((tiles + least - 1) / least);
     const int64_t wgs = kv_split > 0 ? most : std::min<int64_t>(most, paged_slots(k));
     return {(int32_t)wgs, (int32_t)least, kv_split > 0, true};
