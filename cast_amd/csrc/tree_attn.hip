@@ -77,7 +77,8 @@ struct KvSource {
     int32_t store, cap;
     const int32_t *table;
     int64_t table_ld, kpage, vpage;
-    int32_t page_size;
+    int32_t page_size, n_pages;
+    int32_t *bad;   // [batch] workspace: whether a request's prefix names a page outside the pool
 };
 enum { kSrcConcat = 0, kSrcStore = 1, kSrcPages = 2 };   // the kernels' instances by layout
 
@@ -512,8 +513,8 @@ struct KvView {
 // The pages of one request's prefix, for a workgroup that walks keys from
 // k_begin (a multiple of 64) on: lane j holds the id of the page of keys
 // [64 j, 64 j + 64) behind `from`, loaded 64 tiles ahead, so that a tile's
-// fetch finds its page without a round trip.  The ids of accepted requests
-// were checked (page_check_kernel).
+// fetch finds its page without a round trip.  The ids of the request have been
+// looked over (reject_bad_pages).
 template <typename T>
 struct PageView {
     const int32_t *row;
@@ -921,6 +922,33 @@ __device__ bool sk_next_segment(const AttnArgs &a, WorkCursor &cur, Unit &u, con
     return false;
 }
 
+// Whether the unit's request names a page outside the pool: every workgroup of
+// a request looks over all ids of its prefix, so that all of them, and the
+// combine kernel by their word in a.kv.bad, reject it alike.  The workgroup's
+// rows are then zeros with lse = -inf.  (A kernel in front that did this took
+// 4.6 us of a call's 75 to 93, and a launch.)
+__device__ bool reject_bad_pages(const AttnArgs &a, const Unit &u) {
+    const Seq &s = u.sq;
+    const int n = s.S > 0 ? a.by_page.div(s.S - 1) + 1 : 0;
+    const int32_t *row = a.kv.table + (int64_t)s.b * a.kv.table_ld;
+    bool bad = false;
+    for (int i = threadIdx.x; i < n; i += blockDim.x) bad |= (uint32_t)row[i] >= (uint32_t)a.kv.n_pages;
+    bad = __syncthreads_or(bad);
+    if (threadIdx.x == 0) {
+        a.kv.bad[s.b] = bad;
+        if (bad) raise_flag(a.status, CAST_FLAG_BAD_PAGE);
+    }
+    if (!bad) return false;
+    const int r0 = u.rb * a.rows_wg, rows = min(s.P * a.G - r0, a.rows_wg), chunks = a.D * a.esz / 16;
+    for (int i = threadIdx.x; i < rows * chunks; i += blockDim.x) {
+        const int r = r0 + i / chunks, t = a.by_G.div(r), tok = s.q0 + t, head = u.h * a.G + r - t * a.G;
+        char *op = static_cast<char *>(a.out) + ((int64_t)tok * a.o_tok + (int64_t)head * a.o_head) * a.esz;
+        reinterpret_cast<u32x4 *>(op)[i % chunks] = u32x4{};
+        if (a.lse && i % chunks == 0) a.lse[(int64_t)tok * a.Hq + head] = -INFINITY;
+    }
+    return true;
+}
+
 // The first piece of work of the calling workgroup, after the batch
 // prologue; false when it has none (or the batch was rejected).  Batches of
 // up to 64 requests take the stream-K lanes when the caller asked for them
@@ -1056,6 +1084,8 @@ void tree_attn_mfma_kernel(AttnArgs a) {
     Unit wu;
     WorkCursor cur;
     if (!first_unit<kStreamK>(a, cur, wu, skr)) return;
+    if constexpr (SRC == kSrcPages)
+        if (reject_bad_pages(a, wu)) return;
     const int tid = threadIdx.x;
     const int wave = tid >> 6;
     const int lane = tid & 63;
@@ -1549,6 +1579,8 @@ void tree_attn_f32_kernel(AttnArgs a) {
     Unit wu;
     WorkCursor cur;
     if (!first_unit<SKI>(a, cur, wu, skr)) return;
+    if constexpr (SRC == kSrcPages)
+        if (reject_bad_pages(a, wu)) return;
     const int tid = threadIdx.x;
     const int wave = tid >> 6;
     const int lane = tid & 63;
@@ -2043,6 +2075,7 @@ __global__ __launch_bounds__(256) void tree_attn_combine_kernel(AttnArgs a) {
         if (!find_request(a, tok, true, sq, i)) return;
     }
     if (sq.ns <= 1) return;
+    if (a.kv.bad && a.kv.bad[sq.b]) return;   // (the attention kernel wrote the rows of a request with a bad page)
     if (sq.part_off + (int64_t)sq.ns * sq.P > a.part_rows) return;
     const int64_t lstride = (int64_t)sq.P * a.Hq, xstride = lstride * D;
     const int hend = min(a.Hq, h0 + hpg);
@@ -2858,32 +2891,8 @@ extern "C" int cast_tree_attn_store_fwd(const void *q, const void *k_store, cons
 }
 
 // --------------------------------------------------------------------------
-// The prefix in pages.  A kernel in front looks every page id of a request
-// over, so that the attention and the combine kernels reject it alike.
+// The prefix in pages.
 // --------------------------------------------------------------------------
-namespace cast {
-// Request b's prefix length, or -1 where it names a page outside the pool.
-__global__ __launch_bounds__(64) void page_check_kernel(const int32_t *table, int64_t table_ld, int32_t n_pages, int32_t cap,
-                                                        FastDiv by_page, const int32_t *prefix_len, int32_t *checked,
-                                                        int32_t *status) {
-    const int b = blockIdx.x;
-    const int S = prefix_len[b];
-    bool bad = false;
-    if (S > 0 && S <= cap) {
-        const int n = by_page.div(S - 1) + 1;
-        for (int i = threadIdx.x; i < n; i += 64) {
-            const int id = table[(int64_t)b * table_ld + i];
-            bad |= id < 0 || id >= n_pages;
-        }
-    }
-    bad = __any(bad);
-    if (threadIdx.x == 0) {
-        if (bad) raise_flag(status, CAST_FLAG_BAD_PAGE);
-        checked[b] = bad ? -1 : S;
-    }
-}
-}  // namespace cast
-
 // (stream-K has no instances for pages: as for other calls without one, no split)
 static int32_t paged_split(int32_t kv_split) { return kv_split == kSplitStreamK ? -1 : kv_split; }
 
@@ -2935,26 +2944,18 @@ extern "C" int cast_tree_attn_paged_fwd(const void *q, const void *k_pages, cons
     s.kpage = kp_page;
     s.vpage = vp_page;
     s.page_size = page_size;
+    s.n_pages = n_pages;
+    s.bad = page_table ? static_cast<int32_t *>(workspace) : nullptr;   // (no table: no prefix, and a store of no slots)
     const size_t head = batch > 0 ? align256((size_t)batch * sizeof(int32_t)) : 0;
-    int32_t *checked = static_cast<int32_t *>(workspace);
-    auto run = [&](int stages) {
-        return tree_attn_run(q, s, out, lse, cu_q, nullptr, stages ? checked : prefix_len, pack_len, mask, mask_words,
-                             batch, total_q, total_kv, num_q_heads, num_kv_heads, head_dim, q_tok, q_head, o_tok, o_head,
-                             dtype, sm_scale, paged_split(kv_split), static_cast<char *>(workspace) + head,
-                             workspace_bytes - head, status, stream, stages);
-    };
-    // the arguments first: no kernel runs on ones the attention refuses
     if (batch > 0 && total_q > 0) {
         if (!workspace) return CAST_ERR_NULL_POINTER;
         if (workspace_bytes < head) return CAST_ERR_WORKSPACE;
         if (reinterpret_cast<uintptr_t>(workspace) & 255) return CAST_ERR_ALIGNMENT;
     }
-    const int st = run(0);
-    if (st != CAST_OK || batch == 0 || total_q == 0) return st;
-    page_check_kernel<<<batch, 64, 0, reinterpret_cast<hipStream_t>(stream)>>>(
-        page_table, table_ld, n_pages, s.cap, fast_div((uint32_t)page_size), prefix_len, checked, status);
-    if (hipGetLastError() != hipSuccess) return CAST_ERR_HIP;
-    return run(kStageAttn | kStageCombine);
+    return tree_attn_run(q, s, out, lse, cu_q, nullptr, prefix_len, pack_len, mask, mask_words, batch, total_q, total_kv,
+                         num_q_heads, num_kv_heads, head_dim, q_tok, q_head, o_tok, o_head, dtype, sm_scale,
+                         paged_split(kv_split), static_cast<char *>(workspace) + head, workspace_bytes - head, status,
+                         stream, kStageAttn | kStageCombine);
 }
 
 // --------------------------------------------------------------------------

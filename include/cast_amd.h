@@ -465,13 +465,13 @@ size_t cast_paged_attn_workspace_size(int32_t batch, int32_t max_pages, int32_t 
  * results as over a store that holds the same tokens.
  *   page_size  a multiple of 64, or any size where max_pages is 1; n_pages
  *            bounds the ids (a request whose prefix names another page is
- *            rejected: CAST_FLAG_BAD_PAGE and _BAD_OFFSETS)
+ *            rejected: CAST_FLAG_BAD_PAGE)
  *   total_kv a bound on sum_b (prefix_len[b] + pack_len[b])
  *   workspace  cast_tree_attn_paged_workspace_size(...) bytes, 256-byte
- *            aligned, always needed (the checked lengths lie in it)
+ *            aligned, always needed (a word per request says whether its
+ *            pages are good)
  *   kv_split CAST_SPLIT_STREAM runs unsplit
- * A kernel in front checks the page ids.  Head dims and alignment that take
- * the scalar kernel elsewhere are refused here.
+ * Alignment and sizes that take the scalar kernel elsewhere are refused here.
  * ------------------------------------------------------------------- */
 int cast_tree_attn_paged_fwd(const void *q, const void *k_pages, const void *v_pages,
                              const int32_t *page_table, int64_t table_ld, int32_t max_pages,
