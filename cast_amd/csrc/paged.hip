@@ -211,8 +211,8 @@ __global__ __launch_bounds__(kPagedThreads) void paged_append_kernel(PagedAppend
     u32x4 x{}, y{};
     auto load = [&](int64_t src) __attribute__((always_inline)) {
         if (!live) return;
-        x = *reinterpret_cast<const u32x4 *>(rows + src * row_step);
-        if (paired) y = *reinterpret_cast<const u32x4 *>(rows + src * row_step + far);
+        x = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(rows + src * row_step));   // (read once: 83.5 -> 80 us for 13k tokens)
+        if (paired) y = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(rows + src * row_step + far));
     };
     auto put = [&](const PagedRow &r) __attribute__((always_inline)) {
         char *to, *also = nullptr;   // also: k_out

@@ -350,18 +350,18 @@ void paged_attn_kernel(PagedAttnArgs a) {
         }
     };
 
-    // ---- page ids.  Without ANY a 16-key block lies within one page: lane
-    // 2 i + t (KB = 2) or i (KB = 1) holds the id of block t of tile i0 + i.
+    // ---- page ids, kGroup tiles of them in the lanes of a register: without
+    // ANY, where a 16-key block lies within one page, one a block, with it one a
+    // key; the next group's are loaded a group ahead.
+    constexpr int kIds = ANY ? WK : KB, kGroup = 64 / kIds;
     auto seen = [&](const Piece &c, int key) __attribute__((always_inline)) { return min(max(key, c.start), c.len - 1); };
-    auto page_id = [&](const Piece &c, int key, bool &bad) __attribute__((always_inline)) {   // of a visible key; always a page of the pool
+    auto load_ids = [&](const Piece &c, int i0, bool &bad) __attribute__((always_inline)) {   // of the group at tile i0
+        if (i0 >= c.nt || c.len == 0) return 0;
+        const int i = min(i0 + lane / kIds, c.nt - 1);
+        const int key = seen(c, c.key0 + i * TK + lane % kIds * (WK / kIds));
         const int id = a.table[(int64_t)c.b * a.table_ld + a.by_page.div(key)];
         bad |= id < 0 || id >= a.n_pages;
-        return min(max(id, 0), a.n_pages - 1);
-    };
-    auto load_ids = [&](const Piece &c, int i0, bool &bad) __attribute__((always_inline)) {
-        if (ANY || c.len == 0) return 0;
-        const int i = min(i0 + lane / KB, c.nt - 1);
-        return page_id(c, seen(c, c.key0 + i * TK + (lane % KB) * 16), bad);
+        return min(max(id, 0), a.n_pages - 1);   // always a page of the pool
     };
 
     struct Tile {
@@ -389,8 +389,8 @@ void paged_attn_kernel(PagedAttnArgs a) {
 #pragma unroll
         for (int e = 0; e < VW; ++e) t.v[j][c][e] = y[e];
     };
-    // tile i of the piece (its ids in `ids`, unless ANY)
-    auto load_tile = [&](Tile &t, const Piece &cur, int i, int ids, bool &bad) __attribute__((always_inline)) {
+    // tile i of the piece, its ids in `ids`
+    auto load_tile = [&](Tile &t, const Piece &cur, int i, int ids) __attribute__((always_inline)) {
         if (ANY && (cur.len == 0 || i >= cur.nt)) return;
         const char *kbase = static_cast<const char *>(a.k) + (int64_t)cur.h * a.kp_head;
         const char *vbase = static_cast<const char *>(a.v) + (int64_t)cur.h * a.vp_head;
@@ -403,7 +403,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
                 // (no branch: a tile past the piece's last is a load of nothing)
                 const int kc = max(seen(cur, kb), 0), off = kb - a.by_page.div(kc) * a.page_size;
                 const int keys = i < cur.nt && kb + 16 > cur.start ? cur.len - kb : 0;
-                const int64_t id = __builtin_amdgcn_readlane(ids, (i % (64 / KB)) * KB + t16);
+                const int64_t id = __builtin_amdgcn_readlane(ids, i % kGroup * KB + t16);
                 const __amdgpu_buffer_rsrc_t kr = block(kbase + id * a.kp_page + off * a.kp_tok, keys, a.kp_tok);
                 const __amdgpu_buffer_rsrc_t vr = block(vbase + id * a.vp_page + off * a.vp_tok, keys, a.vp_tok);
 #pragma unroll
@@ -420,10 +420,9 @@ void paged_attn_kernel(PagedAttnArgs a) {
                     }
             } else {
                 // every key's own page; keys that are not seen are clamped into those that are
-                const int key = seen(cur, kb + l16);
-                const int id = page_id(cur, key, bad), off = key - a.by_page.div(key) * a.page_size;
-                auto row_at = [&](const char *pool, int64_t page, int64_t tok, int from) __attribute__((always_inline)) {
-                    return pool + (int64_t)__shfl(id, from) * page + (int64_t)__shfl(off, from) * tok;
+                auto row_at = [&](const char *pool, int64_t page, int64_t tok, int in) __attribute__((always_inline)) {
+                    const int key = seen(cur, kb + in), off = key - a.by_page.div(key) * a.page_size;
+                    return pool + (int64_t)__shfl(ids, i % kGroup * WK + 16 * t16 + in) * page + (int64_t)off * tok;
                 };
 #pragma unroll
                 for (int y = 0; y < 2; ++y) {
@@ -603,22 +602,24 @@ void paged_attn_kernel(PagedAttnArgs a) {
     Tile even;
     bool bad = false;
     Piece cur = piece(p, b, base);
-    int ids = load_ids(cur, 0, bad);
+    int ids = load_ids(cur, 0, bad), ahead = load_ids(cur, kGroup, bad);
     load_q(cur);
-    if (!ANY) load_tile(even, cur, 0, ids, bad);
+    if (!ANY) load_tile(even, cur, 0, ids);
     for (;;) {
-    if (ANY) load_tile(even, cur, 0, ids, bad);
+    if (ANY) load_tile(even, cur, 0, ids);
     const int p_next = uni(p + cur.nt + (cur.last ? cost : 0));
     const bool more = p_next < p_end;
     bool bad_next = false;
-    int ids_next = 0;
+    int ids_next = 0, ahead_next = 0;
     if (more) {
         const int after = base + (paged_req(a, TK, __builtin_amdgcn_readlane(len_l, b - b0)).tiles + cost) * per;
         if (p_next >= after) {
             base = after;
             if (++b == b0 + 64) lengths(b);
         }
-        ids_next = load_ids(piece(p_next, b, base), 0, bad_next);
+        const Piece next = piece(p_next, b, base);
+        ids_next = load_ids(next, 0, bad_next);
+        ahead_next = load_ids(next, kGroup, bad_next);
     }
 #pragma unroll
     for (int n = 0; n < NA; ++n) acc[n] = floatx4{};
@@ -632,16 +633,17 @@ void paged_attn_kernel(PagedAttnArgs a) {
                 for (int i = 0;;) {
                     use_tile(even, cur, i);
                     if (++i >= cur.nt) break;
-                    load_tile(even, cur, i, ids, bad);
+                    if (i % kGroup == 0) ids = ahead, ahead = load_ids(cur, i + kGroup, bad);
+                    load_tile(even, cur, i, ids);
                 }
             }
             for (int i = kAhead ? 0 : cur.nt; i < cur.nt; i += 2) {
                 Tile odd;
-                load_tile(odd, cur, i + 1, ids, bad);
+                load_tile(odd, cur, i + 1, ids);
                 use_tile(even, cur, i);
                 if (i + 1 >= cur.nt) break;
-                if (!ANY && (i + 2) % (64 / KB) == 0) ids = load_ids(cur, i + 2, bad);
-                load_tile(even, cur, i + 2, ids, bad);
+                if ((i + 2) % kGroup == 0) ids = ahead, ahead = load_ids(cur, i + 2 + kGroup, bad);
+                load_tile(even, cur, i + 2, ids);
                 use_tile(odd, cur, i + 1);
             }
             if (F32 || again) break;
@@ -667,18 +669,18 @@ void paged_attn_kernel(PagedAttnArgs a) {
             m = -INFINITY;
             l = 0.f;
             again = true;
-            ids = load_ids(cur, 0, bad);
-            load_tile(even, cur, 0, ids, bad);
+            ids = load_ids(cur, 0, bad), ahead = load_ids(cur, kGroup, bad);
+            load_tile(even, cur, 0, ids);
         }
     }
     const Piece done = cur;
     const bool wbad = __any(bad);
     if (more) {
         cur = piece(p_next, b, base);
-        ids = ids_next;
+        ids = ids_next, ahead = ahead_next;
         bad = bad_next;
         load_q(cur);
-        if (!ANY) load_tile(even, cur, 0, ids, bad);
+        if (!ANY) load_tile(even, cur, 0, ids);
     }
 
     // ---- join the four waves
