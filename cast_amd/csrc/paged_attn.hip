@@ -449,7 +449,9 @@ void paged_attn_kernel(PagedAttnArgs a) {
         }
     };
 
+    // a score's base-2 exponent is the product (capped: the tanh) times to_log2
     const float inv_cap = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
+    const float to_log2 = a.softcap > 0.f ? a.softcap * kPLog2e : a.scale;
     floatx4 acc[NA];
     float m, l;
     bool again;   // see below
@@ -458,10 +460,14 @@ void paged_attn_kernel(PagedAttnArgs a) {
         const bool edge = kt < cur.start || kt + WK > cur.len;
         float p[KB][4];
         __builtin_amdgcn_sched_barrier(0);   // (in this order: a tile's registers, not two stages')
-        // ---- scores, base 2
+        // ---- scores, scaled where their exponent is taken (one rounding)
 #pragma unroll
         for (int t16 = 0; t16 < KB; ++t16) {
-            floatx4 s4 = floatx4{};
+            // (fp32: two sums of every second product, half the roundings and half the wait)
+            constexpr int NS = F32 ? 2 : 1;
+            floatx4 sum[NS];
+#pragma unroll
+            for (int e = 0; e < NS; ++e) sum[e] = floatx4{};
 #pragma unroll
             for (int c = 0; c < KC; ++c) {
                 // words of chunk pair (c & ~1, c | 1): the loads left the first
@@ -481,13 +487,18 @@ void paged_attn_kernel(PagedAttnArgs a) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const uint32_t kw = kx[e];   // (a bit cast of the element itself reads element 0)
-                        s4 = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, kw),
-                                                                  __builtin_bit_cast(float, qraw[c][e]), s4, 0, 0, 0);
+                        sum[e & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, kw),
+                                                                          __builtin_bit_cast(float, qraw[c][e]), sum[e & 1], 0, 0, 0);
                     }
                 } else {
                     const u32x4 qx = {qraw[c][0], qraw[c][1], qraw[c][2], qraw[c][3]};
-                    s4 = E::mma16(__builtin_bit_cast(typename E::vec8, kx), __builtin_bit_cast(typename E::vec8, qx), s4);
+                    sum[0] = E::mma16(__builtin_bit_cast(typename E::vec8, kx), __builtin_bit_cast(typename E::vec8, qx), sum[0]);
                 }
+            }
+            floatx4 s4 = sum[0];
+            if constexpr (F32) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s4[r] = sum[0][r] + sum[1][r];
             }
             if (a.softcap > 0.f) {
 #pragma unroll
@@ -498,11 +509,11 @@ void paged_attn_kernel(PagedAttnArgs a) {
                     const float far = 1.f - 2.f / (__builtin_amdgcn_exp2f(x * (2.f * kPLog2e)) + 1.f);
                     const float poly = fmaf(fmaf(fmaf(62.f / 2835.f, x2, -17.f / 315.f), x2, 2.f / 15.f), x2, -1.f / 3.f);
                     const float near = fmaf(x * x2, poly, x);
-                    p[t16][r] = (x2 < 0.0625f ? near : far) * (a.softcap * kPLog2e);
+                    p[t16][r] = x2 < 0.0625f ? near : far;
                 }
             } else {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) p[t16][r] = s4[r] * a.scale;
+                for (int r = 0; r < 4; ++r) p[t16][r] = s4[r];
             }
         }
         if (edge) {
@@ -523,14 +534,14 @@ void paged_attn_kernel(PagedAttnArgs a) {
                     }
                 }
         }
-        // ---- running maximum: moved for all columns at once, when any needs it
+        // ---- running maximum (base 2): moved for all columns at once, when any needs it
         float top = p[0][0];
 #pragma unroll
         for (int t16 = 0; t16 < KB; ++t16)
 #pragma unroll
             for (int r = 0; r < 4; ++r) top = fmaxf(top, p[t16][r]);
-        if (__any(top > m)) {
-            const float mn = fmaxf(m, quad_max(top));
+        if (__any(top * to_log2 > m)) {
+            const float mn = fmaxf(m, quad_max(top) * to_log2);
             const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
             m = mn;
             l *= alpha;
@@ -542,7 +553,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
         for (int t16 = 0; t16 < KB; ++t16)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                p[t16][r] = __builtin_amdgcn_exp2f(p[t16][r] - ms);
+                p[t16][r] = __builtin_amdgcn_exp2f(fmaf(p[t16][r], to_log2, -ms));
                 l += p[t16][r];
             }
         // ---- O^T += V^T P^T
