@@ -56,7 +56,14 @@ constexpr int kPWaves = 4;
 // and 35.9 us for 0 to 3; 64 of 300 to 8k at D = 128, bf16, 219.5, 222, 225, 230.
 constexpr int piece_cost(int D) { return D == 64 ? 2 : 1; }
 constexpr int kLensLds = 1024;           // batches whose lengths a workgroup keeps in LDS for its schedule
-constexpr int kMinTiles = 2;             // fewest key tiles of a workgroup's stretch, unless the caller says
+// Fewest key tiles of a piece, unless the caller says: one request of 2k keys
+// over 8 KV heads 8.9, 10.8, 12.3 and 16.4 us (without the join) at 1, 2, 4, 8.
+constexpr int kMinTiles = 1;
+// Tiles a workgroup should have before a CU gets a second one, where units are
+// fewer than CUs: one request of 32k keys 24.1 + 4.0 us (attention, join) on 256
+// workgroups of 8 tiles, 24.8 + 5.0 on 512 of 4.  (Units of their own are better
+// spread: 200 requests of up to 1k keys, 4 KV heads, 35 us on 768, 37.6 on 440.)
+constexpr int kFewTiles = 8;
 
 struct PagedAttnArgs {
     const void *q, *k, *v;
@@ -69,6 +76,7 @@ struct PagedAttnArgs {
     int32_t n_pages, page_size, batch, Hq, Hkv, G, rbs, D, cap, window;  // cap: slots a table row covers
     FastDiv by_page;    // division by page_size
     int32_t wgs;        // workgroups of the attention kernel
+    int32_t cus;        // CUs of the device
     int32_t least;      // fewest tiles of a piece; 0: one workgroup per unit, no pieces
     int32_t cut;        // pieces of exactly `least` tiles, as the caller says
     int32_t prows;      // rows of a partial: min(16, G)
@@ -161,8 +169,8 @@ __device__ __forceinline__ int splits_of(int tiles, int c) {
 }
 struct Stretches {
     int W, q, r;
-    __device__ __forceinline__ Stretches(const PagedAttnArgs &a, int all) {
-        W = min(a.wgs, (int)(((uint32_t)all + (uint32_t)a.least - 1) / (uint32_t)a.least));
+    __device__ __forceinline__ Stretches(int wgs, int least, int all) {
+        W = min(wgs, (int)(((uint32_t)all + (uint32_t)least - 1) / (uint32_t)least));
         q = (int)((uint32_t)all / (uint32_t)W);
         r = all - q * W;
     }
@@ -216,7 +224,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
             const int n = paged_req(a, TK, len_l).tiles;
             return k + lane >= a.batch ? 0 : (c ? splits_of(n, c) : n + piece_cost(D)) * per;
         };
-        int all = 0, c = a.cut ? a.least : 0, items = 0;
+        int all = 0, c = a.cut ? a.least : 0, items = 0, wgs = a.wgs;
         for (;;) {
             int n = 0;
 #pragma unroll 1
@@ -227,7 +235,9 @@ void paged_attn_kernel(PagedAttnArgs a) {
             }
             if (c == 0) {
                 all = n;
-                c = max(a.least, (int)(((uint32_t)(all - a.batch * per * piece_cost(D)) + (uint32_t)a.wgs - 1) / (uint32_t)a.wgs));
+                const int tiles = all - a.batch * per * piece_cost(D);
+                if (a.batch * per < a.cus) wgs = min(wgs, max(a.cus, tiles / kFewTiles));
+                c = max(a.least, (int)(((uint32_t)tiles + (uint32_t)wgs - 1) / (uint32_t)wgs));
             } else if (n <= a.wgs) {
                 items = n;
                 break;
@@ -239,7 +249,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
                 c += c >> 3;
             }
         }
-        const Stretches st(a, c ? a.least : all);
+        const Stretches st(wgs, a.least, c ? a.least : all);
         if (x >= (c ? items : st.W)) return;
         const int at = c ? x : st.first(x);
 #pragma unroll 1
@@ -882,30 +892,33 @@ static bool paged_any(int32_t page_size, int32_t max_pages) { return page_size %
 // Workgroups of kernel k that the current device holds at once (an MI355X's
 // 256 CUs, one each, where no device is visible), looked up once per (device,
 // kernel).
-static int paged_slots(const PagedKernel &k) {
+struct PagedDevice {
+    int slots, cus;
+};
+static PagedDevice paged_slots(const PagedKernel &k) {
     struct Entry {
         int dev;
         const void *fn;
-        int n;
+        PagedDevice d;
     };
     static std::mutex mu;
     static Entry cache[128];
     static int used = 0;
     int dev = -1;
-    if (hipGetDevice(&dev) != hipSuccess) return 256;
+    if (hipGetDevice(&dev) != hipSuccess) return {256, 256};
     std::lock_guard<std::mutex> lock(mu);
     for (int i = 0; i < used; ++i)
-        if (cache[i].dev == dev && cache[i].fn == k.fn) return cache[i].n;
+        if (cache[i].dev == dev && cache[i].fn == k.fn) return cache[i].d;
     int n = 0, cus = 0;
     if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, k.fn, kPWaves * 64, 0) != hipSuccess || n < 1) n = 1;
     if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus < 1) cus = 256;
-    n *= cus;
-    if (used < 128) cache[used++] = Entry{dev, k.fn, n};
-    return n;
+    const PagedDevice d{n * cus, cus};
+    if (used < 128) cache[used++] = Entry{dev, k.fn, d};
+    return d;
 }
 
 struct PagedPlan {
-    int32_t wgs, least, cut;   // as PagedAttnArgs
+    int32_t wgs, least, cut, cus;   // as PagedAttnArgs
     bool fits;            // tile indices fit 31 bits for any lengths
 };
 static PagedPlan paged_plan(int32_t batch, int32_t max_pages, int32_t page_size, int32_t Hq, int32_t Hkv, int32_t D,
@@ -916,11 +929,12 @@ static PagedPlan paged_plan(int32_t batch, int32_t max_pages, int32_t page_size,
     if (window > 0 && window < keys) keys = (int64_t)window + k.tile - 1;   // (a window may start inside a tile)
     const int64_t tiles = (keys + k.tile - 1) / k.tile;
     const int64_t least = kv_split > 0 ? ((int64_t)kv_split + k.tile - 1) / k.tile : kMinTiles;
-    if (kv_split < 0 || tiles <= least) return {units > INT_MAX ? 0 : (int32_t)units, 0, 0, units <= INT_MAX};
-    if (units > INT_MAX / (tiles + piece_cost(64))) return {0, 0, 0, false};
+    if (kv_split < 0 || tiles <= least) return {units > INT_MAX ? 0 : (int32_t)units, 0, 0, 0, units <= INT_MAX};
+    if (units > INT_MAX / (tiles + piece_cost(64))) return {0, 0, 0, 0, false};
     const int64_t most = units * ((tiles + least - 1) / least);
-    const int64_t wgs = kv_split > 0 ? most : std::min<int64_t>(most, paged_slots(k));
-    return {(int32_t)wgs, (int32_t)least, kv_split > 0, true};
+    const PagedDevice d = paged_slots(k);
+    const int64_t wgs = kv_split > 0 ? most : std::min<int64_t>(most, d.slots);
+    return {(int32_t)wgs, (int32_t)least, kv_split > 0, d.cus, true};
 }
 static size_t p_align256(size_t x) { return (x + 255) & ~(size_t)255; }
 struct PagedParts {
@@ -1019,6 +1033,7 @@ extern "C" int cast_paged_attn_fwd(const void *q, const void *k_pages, const voi
     a.wgs = p.wgs;
     a.least = p.least;
     a.cut = p.cut;
+    a.cus = p.cus;
     a.prows = std::min(a.G, 16);
     a.softcap = softcap;
     a.scale = softcap > 0.f ? sm_scale : sm_scale * kPLog2e;

@@ -101,7 +101,7 @@ def test_workspace_size(lib):
         B, pages, ps, Hq, Hkv, D, w, dt, split)
     assert size() > 0 and size(split=-1) == 0
     assert size(pages=1) == 0                       # too short to split
-    assert size(w=100) == 0                         # and so is the window
+    assert size(w=1) == 0                           # and so is the window
     assert size(Hq=7) == 0 and size(D=100) == 0 and size(dt=2) == 0 and size(B=0) == 0
     assert size(split=128) > size(split=256) > 0
 
