@@ -174,6 +174,9 @@ __global__ __launch_bounds__(kPagedThreads) void paged_append_kernel(PagedAppend
         const int S = a.seq_len[b];
         int root, n;
         int32_t flags = 0;
+        // (where offsets decrease, rows may have gone to another request)
+        if (a.cu_q && !a.path)
+            for (int i = threadIdx.x; i < a.batch; i += kPagedThreads) flags |= a.cu_q[i + 1] < a.cu_q[i] ? CAST_FLAG_BAD_OFFSETS : 0;
         if (!paged_request(a, b, root, n)) {
             flags = CAST_FLAG_BAD_OFFSETS;
         } else {

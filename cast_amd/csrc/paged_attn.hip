@@ -460,7 +460,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
     };
 
     // a score's base-2 exponent is the product (capped: the tanh) times to_log2
-    const float inv_cap = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
+    const float inv_cap = a.softcap > 0.f ? fminf(a.scale / a.softcap, 0x1.fffffep127f) : 0.f;
     const float to_log2 = a.softcap > 0.f ? a.softcap * kPLog2e : a.scale;
     floatx4 acc[NA];
     float m, l;

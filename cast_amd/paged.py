@@ -132,11 +132,11 @@ def paged_append(k, v, k_pages, v_pages, page_table, seq_len, cu_q=None, *, q=No
     H_q = 0
     if q is not None:
         H_q = q.shape[1] if q.dim() == 3 else 0
-        q_in = _rows("q", q, H_q, pools, total)
+        q = _rows("q", q, H_q, pools, total) if q_out is not q else _output("q", q, H_q, pools, total)
         assert H_q > 0 and H_q % H_kv == 0
         q_out = torch.empty_like(q, memory_format=torch.contiguous_format) if q_out is None else \
             _output("q_out", q_out, H_q, pools, total)
-        q_in, q_st, q_to, qo_st = q_in.data_ptr(), q_in.stride()[:2], q_out.data_ptr(), q_out.stride()[:2]
+        q_in, q_st, q_to, qo_st = q.data_ptr(), q.stride()[:2], q_out.data_ptr(), q_out.stride()[:2]
     elif q_out is not None:
         raise ValueError("q_out without q")
     else:

@@ -286,6 +286,8 @@ def begin_verify(buf_k, buf_v, store_len, roots, trees, seq_lens, device=None, p
     cap = int(buf_k[0].shape[2])
     if page_table is not None:
         page_table = _page_rows(page_table, B, dev)
+        if cap % 64 and page_table.shape[1] > 1:
+            raise ValueError("a verify pass over pages needs a page size that is a multiple of 64")
         cap *= int(page_table.shape[1])
     if max(store_len) > cap:
         raise ValueError("store_len exceeds the store capacity")

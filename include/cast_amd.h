@@ -403,7 +403,7 @@ int cast_build_trees_uniform(const int64_t *top_idx, const void *top_lp, int32_t
  * Rotation, q and k_out take one layer and no path.  A row whose slot, page
  * id or position is out of range is skipped whole (its pages, q_out and
  * k_out rows keep what they held); *status gets CAST_FLAG_BAD_OFFSETS,
- * _BAD_PAGE or _BAD_POSITION.  Two rows that the tables send to one slot
+ * _BAD_PAGE or _BAD_POSITION.  Where cu_q decreases, every new_len is seq_len.  Two rows that the tables send to one slot
  * leave either's elements.
  * ------------------------------------------------------------------- */
 int cast_paged_append(const void *const *k, const void *const *v, void *const *k_pages,

@@ -425,3 +425,85 @@ def test_prompts_then_decode_steps_match_a_dense_cache(gpu):
             ref = OP.attention(qr[b:b + 1].cpu(), dense[b][0].transpose(0, 1)[None], dense[b][1].transpose(0, 1)[None],
                                [[0]], [n])
             check_attention(out[b:b + 1], lse[b:b + 1], ref, torch.bfloat16, n, D)
+
+
+def test_unaligned_rows_are_copied_and_kept(gpu):
+    # inputs that start off 16 bytes are copied for the call; what the call allocates afterwards must not take the
+    # copies' memory
+    from cast_amd import paged_append
+    g = torch.Generator().manual_seed(0)
+    table = torch.tensor([[0, 1]], dtype=torch.int32, device=gpu)
+    big = [torch.randn(20 * h * 64 + 1, generator=g).to(torch.bfloat16).to(gpu) for h in (4, 2, 2)]
+    q, k, v = (x[1:].view(20, h, 64) for x, h in zip(big, (4, 2, 2)))
+    pools = [torch.zeros((2, 2, 16, 64), dtype=torch.bfloat16, device=gpu) for _ in range(2)]
+    for _ in range(5):
+        out, n = paged_append(k, v, *pools, table, [0], [0, 20], q=q, check=True)
+        assert torch.equal(out, q) and n.tolist() == [20]
+        for pool, x in zip(pools, (k, v)):
+            assert torch.equal(pool.transpose(1, 2).reshape(32, 2, 64)[:20], x)
+            pool.zero_()
+    with pytest.raises(ValueError, match="aligned"):
+        paged_append(k, v, *pools, table, [0], [0, 20], q=q, q_out=q)
+    with pytest.raises(ValueError, match="expanded"):
+        paged_append(k, v, *pools, table, [0], [0, 20], k_out=torch.zeros((1, 2, 64), dtype=torch.bfloat16,
+                                                                          device=gpu).expand(20, 2, 64))
+
+
+def test_decreasing_offsets_leave_every_length(gpu):
+    from cast_amd import paged_append
+    k = torch.zeros((4, 1, 64), dtype=torch.bfloat16, device=gpu)
+    pools = [torch.zeros((3, 1, 16, 64), dtype=torch.bfloat16, device=gpu) for _ in range(2)]
+    table = torch.arange(3, dtype=torch.int32, device=gpu)[:, None]
+    cu = torch.tensor([0, 3, 1, 4], dtype=torch.int32, device=gpu)
+    _, n = paged_append(k, k, *pools, table, torch.tensor([1, 2, 3], dtype=torch.int32, device=gpu), cu)
+    assert n.tolist() == [1, 2, 3]
+
+
+def test_nothing_to_do(gpu):
+    from cast_amd import paged_append, paged_attention
+    pools = [torch.zeros((2, 2, 16, 64), dtype=torch.bfloat16, device=gpu) for _ in range(2)]
+    none = torch.zeros((0, 2, 64), dtype=torch.bfloat16, device=gpu)
+    table = torch.zeros((3, 1), dtype=torch.int32, device=gpu)
+    q, n = paged_append(none, none, *pools, table, [4, 5, 6], [0, 0, 0, 0], q=none[:, :, :], check=True)
+    assert n.tolist() == [4, 5, 6] and q.shape == (0, 2, 64)
+    out, lse = paged_attention(none, *pools, table[:0], torch.zeros(0, dtype=torch.int32, device=gpu), return_lse=True)
+    assert out.shape == (0, 2, 64) and lse.shape == (0, 2)
+
+
+def test_two_calls_at_once_on_two_streams(gpu):
+    # different batches in flight on two streams, each with its own workspace: the bits of the calls alone
+    from cast_amd import paged_attention
+    sets = []
+    for seed, lens in ((1, [4000, 100, 2500]), (2, [700] * 40)):
+        kp, vp, table, g = make_cache(gpu, lens, 2, 64, 16, "bf16", seed=seed)
+        q = torch.randn((len(lens), 8, 64), generator=g).to(torch.bfloat16)
+        sets.append((q.to(gpu), kp.to(gpu), vp.to(gpu), table.to(gpu), torch.tensor(lens, dtype=torch.int32, device=gpu)))
+    want = [paged_attention(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(10):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(paged_attention(*sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])
+
+
+def test_the_largest_batch_and_a_tiny_cap(gpu):
+    # 65535 requests (one more is refused), and a cap so small that every score is it
+    from cast_amd import paged_attention
+    B = 65535
+    pools = [torch.ones((1, 1, 16, 64), dtype=torch.bfloat16, device=gpu) for _ in range(2)]
+    pools[1][0, 0, 1] = 3
+    q = torch.ones((B, 1, 64), dtype=torch.bfloat16, device=gpu)
+    lens = (torch.arange(B, device=gpu) % 3).to(torch.int32)
+    table = torch.zeros((1, 1), dtype=torch.int32, device=gpu).expand(B, 1)
+    out = paged_attention(q, *pools, table, lens, check=True)
+    assert torch.equal(out[:, 0, 0].float(), torch.tensor([0.0, 1.0, 2.0], device=gpu)[lens.long()])
+    from cast_amd._lib import CastError
+    with pytest.raises(CastError):
+        paged_attention(torch.cat([q, q[:1]]), *pools, table.new_zeros((B + 1, 1)), torch.cat([lens, lens[:1]]))
+    out, lse = paged_attention(q[:2] * 0, *pools, table[:2], [2, 2], softcap=1e-45, return_lse=True)
+    assert (out == 2).all() and (lse - np.log(2)).abs().max() < 1e-6
