@@ -238,6 +238,10 @@ void paged_attn_kernel(PagedAttnArgs a) {
                 const int tiles = all - a.batch * per * piece_cost(D);
                 if (a.batch * per < a.cus) wgs = min(wgs, max(a.cus, tiles / kFewTiles));
                 c = max(a.least, (int)(((uint32_t)tiles + (uint32_t)wgs - 1) / (uint32_t)wgs));
+                if (a.batch * per > a.wgs) {   // (a piece per unit is too many)
+                    c = 0;
+                    break;
+                }
             } else if (n <= a.wgs) {
                 items = n;
                 break;
