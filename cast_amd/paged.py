@@ -97,6 +97,20 @@ def _output(name, x, heads, pools, total):
     return x
 
 
+_INT32 = (1 << 31) - 1
+
+
+def _workspace(workspace, need, like):
+    """The caller's workspace where it holds `need` bytes, else a new one."""
+    if workspace is not None:
+        _require_on(like.device, workspace=workspace)
+        if not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous")
+        if workspace.numel() * workspace.element_size() >= need:
+            return workspace
+    return like.new_empty(need, dtype=torch.uint8)
+
+
 def _no_overlap(name, t):
     """An output whose elements share memory (an expanded tensor) cannot be written."""
     if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
@@ -150,6 +164,8 @@ def paged_append(k, v, k_pages, v_pages, page_table, seq_len, cu_q=None, *, q=No
         if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype is not torch.float32 or sin.dtype is not torch.float32:
             raise ValueError("cos and sin must both be float32 [max_pos, rot_dim / 2]")
         max_pos, rot_dim = cos.shape[0], 2 * cos.shape[1]
+        if not max_pos:
+            raise ValueError("cos and sin hold no position")
         if not 0 < rot_dim <= D or rot_dim % (32 // esz):
             raise ValueError(f"rot_dim must be a multiple of {32 // esz} up to the head dim {D}, got {rot_dim}")
         if cos.get_device() != pools.index or sin.get_device() != pools.index:
@@ -228,7 +244,8 @@ def paged_attention(q, k_pages, v_pages, page_table, seq_len, sm_scale=None, *, 
     pool return zeros with lse = -inf; ``check=True`` raises.
     """
     lib = _lib.load()
-    kv_split, window = operator.index(kv_split), operator.index(window)
+    # (sizes past 31 bits mean what the largest of them does)
+    kv_split, window = max(-1, min(operator.index(kv_split), _INT32)), min(operator.index(window), _INT32)
     pools = _Pools(k_pages, v_pages, "paged_attention")
     H_kv, D, dev = pools.H_kv, pools.D, pools.device
     if q.dim() != 3:
@@ -248,10 +265,8 @@ def paged_attention(q, k_pages, v_pages, page_table, seq_len, sm_scale=None, *, 
         sm_scale = 1.0 / math.sqrt(D)
     max_pages = page_table.shape[1]
     ws_bytes = _workspace_bytes(pools.index, B, max_pages, pools.page_size, H_q, H_kv, D, window, pools.code, kv_split)
-    if workspace is not None:
-        _require_on(dev, workspace=workspace)
-    if ws_bytes and (workspace is None or workspace.numel() * workspace.element_size() < ws_bytes):
-        workspace = q.new_empty(ws_bytes, dtype=torch.uint8)
+    if ws_bytes or workspace is not None:
+        workspace = _workspace(workspace, ws_bytes, q)
     status = torch.zeros(1, dtype=torch.int32, device=dev) if check else None
     with _lib.on_device(dev):
         st = lib.cast_paged_attn_fwd(
@@ -307,7 +322,7 @@ def paged_tree_attention(q, k_pages, v_pages, page_table, k_pack, v_pack, cu_q, 
     inconsistent lengths: zeros with lse = -inf, and ``check=True`` raises.
     """
     lib = _lib.load()
-    kv_split = operator.index(kv_split)
+    kv_split = max(-_INT32, min(operator.index(kv_split), _INT32))
     pools = _Pools(k_pages, v_pages, "paged_tree_attention")
     H_kv, D, dev = pools.H_kv, pools.D, pools.device
     if pools.n_pages == 0:
@@ -339,10 +354,7 @@ def paged_tree_attention(q, k_pages, v_pages, page_table, k_pack, v_pack, cu_q, 
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(D)
     ws_bytes = _tree_workspace_bytes(pools.index, B, total_q, total_kv, H_q, H_kv, D, pools.code, kv_split)
-    if workspace is not None:
-        _require_on(dev, workspace=workspace)
-    if workspace is None or workspace.numel() * workspace.element_size() < ws_bytes:
-        workspace = q.new_empty(ws_bytes, dtype=torch.uint8)
+    workspace = _workspace(workspace, ws_bytes, q)
     status = torch.zeros(1, dtype=torch.int32, device=dev) if check else None
     with _lib.on_device(dev):
         st = lib.cast_tree_attn_paged_fwd(

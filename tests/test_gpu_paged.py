@@ -507,3 +507,26 @@ def test_the_largest_batch_and_a_tiny_cap(gpu):
         paged_attention(torch.cat([q, q[:1]]), *pools, table.new_zeros((B + 1, 1)), torch.cat([lens, lens[:1]]))
     out, lse = paged_attention(q[:2] * 0, *pools, table[:2], [2, 2], softcap=1e-45, return_lse=True)
     assert (out == 2).all() and (lse - np.log(2)).abs().max() < 1e-6
+
+
+def test_empty_tables_strided_workspaces_and_sizes_past_31_bits(gpu):
+    from cast_amd import paged_append, paged_attention
+    kp, vp, table, g = make_cache(gpu, [300, 17], 2, 64, 16, "bf16")
+    kp, vp, table = kp.to(gpu), vp.to(gpu), table.to(gpu)
+    lens = torch.tensor([300, 17], dtype=torch.int32, device=gpu)
+    q = torch.randn((2, 8, 64), generator=g).bfloat16().to(gpu)
+    # tables of no position rotate nothing: not a way to ask for no rotation
+    before = kp.clone()
+    none = torch.zeros((0, 32), device=gpu)
+    with pytest.raises(ValueError, match="no position"):
+        paged_append(q[:, :2], q[:, :2], kp, vp, table, lens, cos=none, sin=none)
+    assert torch.equal(kp.view(torch.int16), before.view(torch.int16))
+    # a workspace whose bytes do not lie side by side
+    thin = torch.empty(1, dtype=torch.uint8, device=gpu).expand(1 << 26)
+    with pytest.raises(ValueError, match="contiguous"):
+        paged_attention(q, kp, vp, table, lens, workspace=thin)
+    # a window or split past 31 bits is as good as the largest one
+    ref = paged_attention(q, kp, vp, table, lens, kv_split=-1)
+    assert torch.equal(paged_attention(q, kp, vp, table, lens, window=(1 << 32) + 5, kv_split=-1), ref)
+    assert torch.equal(paged_attention(q, kp, vp, table, lens, kv_split=(1 << 32) + 128), ref)
+    assert torch.equal(paged_attention(q, kp, vp, table, lens, kv_split=-(1 << 32) + 128), ref)
