@@ -99,6 +99,23 @@ def load():
     return lib
 
 
+_calls = None
+
+
+def calls():
+    """cast_amd._calls, the paged calls of arguments that need no conversion."""
+    global _calls
+    if _calls is None:
+        load()
+        try:
+            from . import _calls as module
+        except ImportError as e:
+            raise RuntimeError("cast_amd/_calls.so is missing or does not load: build it with "
+                               "`python -m cast_amd.build`") from e
+        _calls = module
+    return _calls
+
+
 def status_string(status):
     try:
         return load().cast_status_string(int(status)).decode()

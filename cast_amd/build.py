@@ -1,9 +1,10 @@
 """Build the HIP libraries for gfx950 with hipcc.
 
-    python -m cast_amd.build            # cast_amd/libcast_amd.so and libcast_bench.so
+    python -m cast_amd.build            # cast_amd/libcast_amd.so, _calls.so and libcast_bench.so
 
 libcast_amd.so (the product, the C ABI of include/cast_amd.h) comes from
-cast_amd/csrc/*.hip; libcast_bench.so (bench.py's measurement aids,
+cast_amd/csrc/*.hip; _calls.so (host code: the paged calls straight from torch
+tensors) from cast_amd/csrc/calls.cpp, linked to it; libcast_bench.so (bench.py's measurement aids,
 cast_amd/csrc/bench/cast_bench.h) from cast_amd/csrc/bench/*.hip.  Compiler
 warnings are printed; a register-budget miss in an attention kernel
 (``-Wpass-failed``: an amdgpu_waves_per_eu target not met) fails the build.
@@ -18,6 +19,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -26,6 +28,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 OUT = PKG / "libcast_amd.so"
 BENCH_OUT = PKG / "libcast_bench.so"
+CALLS_OUT = PKG / "_calls.so"
 ARCH = "gfx950"
 
 HIPCC_FLAGS = [
@@ -91,6 +94,26 @@ def _link(hipcc, objs, out):
     os.replace(str(out) + ".tmp", out)
 
 
+def _build_calls():
+    """cast_amd/_calls.so: host code against torch's headers, linked to libcast_amd.so beside it."""
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+    cxx = os.environ.get("CXX") or shutil.which("g++") or "c++"
+    tmp = str(CALLS_OUT) + ".tmp"
+    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", str(CSRC / "calls.cpp"), "-o", tmp, "-I", str(ROOT / "include"),
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    for inc in [*include_paths(), sysconfig.get_paths()["include"]]:
+        cmd += ["-isystem", inc]
+    for lib in library_paths():
+        cmd += [f"-L{lib}", f"-Wl,-rpath,{lib}"]
+    cmd += ["-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", f"-L{PKG}", f"-l:{OUT.name}", "-Wl,-rpath,$ORIGIN"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"{cxx} failed on calls.cpp:\n{res.stderr}")
+    os.replace(tmp, CALLS_OUT)
+    return res.stderr
+
+
 def _warnings(stderr):
     """hipcc's warnings, without its note that the host pass does not know
     the device-only -packed-fp32-ops feature."""
@@ -125,6 +148,9 @@ def build(verbose: bool = True) -> Path:
     n = len(sources())
     _link(hipcc, [o for _, o, _ in done[:n]], OUT)
     _link(hipcc, [o for _, o, _ in done[n:]], BENCH_OUT)
+    text = _build_calls()
+    if text and verbose:
+        print(f"warnings in calls.cpp:\n{text}", file=sys.stderr)
     return OUT
 
 

@@ -138,6 +138,14 @@ def paged_append(k, v, k_pages, v_pages, page_table, seq_len, cu_q=None, *, q=No
     A row with an invalid slot, page id or position is skipped whole, and its
     request's new_len stays seq_len; ``check=True`` raises.
     """
+    if not check and k_pages.is_cuda:
+        done = _lib.calls().paged_append(k, v, k_pages, v_pages, page_table, seq_len, cu_q, q, cos, sin, positions,
+                                         interleaved, q_out, k_out, new_len, _lib.stream_of(k_pages))
+        if type(done) is tuple:
+            return done
+        if done is not None:
+            _lib.check(done, "cast_paged_append")
+    # (a status to read, a copy to make, or something to refuse)
     lib = _lib.load()
     pools = _Pools(k_pages, v_pages, "paged_append")
     H_kv, D, dev, esz = pools.H_kv, pools.D, pools.device, pools.esz
@@ -243,9 +251,17 @@ def paged_attention(q, k_pages, v_pages, page_table, seq_len, sm_scale=None, *, 
     Requests with a length outside the table or a visible page id outside the
     pool return zeros with lse = -inf; ``check=True`` raises.
     """
-    lib = _lib.load()
     # (sizes past 31 bits mean what the largest of them does)
     kv_split, window = max(-1, min(operator.index(kv_split), _INT32)), min(operator.index(window), _INT32)
+    if not check and k_pages.is_cuda:
+        done = _lib.calls().paged_attention(q, k_pages, v_pages, page_table, seq_len, sm_scale, softcap, window, kv_split,
+                                            return_lse, out, workspace, _lib.stream_of(k_pages))
+        if type(done) is int:
+            _lib.check(done, "cast_paged_attn_fwd")
+        if done is not None:
+            return done
+    # (a status to read, a copy to make, or something to refuse)
+    lib = _lib.load()
     pools = _Pools(k_pages, v_pages, "paged_attention")
     H_kv, D, dev = pools.H_kv, pools.D, pools.device
     if q.dim() != 3:

@@ -1,0 +1,140 @@
+"""The paged calls straight from tensors: taken for arguments that need no
+conversion, with the results of the checked calls, and left to the wrappers
+for all others."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+def setup(gpu, dtype="bf16", B=3, Hq=8, Hkv=2, D=64, ps=16, pages=40, width=10, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    rnd = lambda *s: torch.randn(s, generator=g).to(DT[dtype]).to(gpu)
+    table = torch.randperm(pages, generator=g)[:B * width].view(B, width).int().to(gpu)
+    s = dict(k=rnd(B, Hkv, D), v=rnd(B, Hkv, D), q=rnd(B, Hq, D), kp=rnd(pages, Hkv, ps, D), vp=rnd(pages, Hkv, ps, D),
+             table=table, lens=torch.tensor([5, 130, 77][:B], dtype=torch.int32, device=gpu))
+    ang = torch.rand((200, D // 2), generator=g)
+    return {**s, "cos": ang.cos().to(gpu), "sin": ang.sin().to(gpu)}
+
+
+def stream(t):
+    from cast_amd import _lib
+    return _lib.stream_of(t)
+
+
+def direct_append(s, **over):
+    from cast_amd import _lib
+    a = dict(k=s["k"], v=s["v"], kp=s["kp"], vp=s["vp"], table=s["table"], lens=s["lens"], cu=None, q=s["q"], cos=s["cos"],
+             sin=s["sin"], pos=None, inter=False, q_out=None, k_out=None, new_len=None)
+    a.update(over)
+    return _lib.calls().paged_append(*a.values(), stream(s["kp"]))
+
+
+def direct_attention(s, **over):
+    from cast_amd import _lib
+    a = dict(q=s["q"], kp=s["kp"], vp=s["vp"], table=s["table"], lens=s["lens"], scale=None, cap=0.0, window=0, split=0,
+             lse=False, out=None, ws=None)
+    a.update(over)
+    return _lib.calls().paged_attention(*a.values(), stream(s["kp"]))
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("inter", [False, True])
+def test_append_is_the_checked_call(gpu, dtype, inter):
+    from cast_amd import paged_append
+    one, two = setup(gpu, dtype), setup(gpu, dtype)
+    pos = torch.tensor([3, 199, 0], dtype=torch.int32, device=gpu)
+    for kw in (dict(), dict(q="q"), dict(q="q", cos="cos", sin="sin", positions=pos), dict(cos="cos", sin="sin")):
+        get = lambda s: {n: s[x] if isinstance(x, str) else x for n, x in kw.items()}
+        got = paged_append(one["k"], one["v"], one["kp"], one["vp"], one["table"], one["lens"], interleaved=inter, **get(one))
+        want = paged_append(two["k"], two["v"], two["kp"], two["vp"], two["table"], two["lens"], interleaved=inter, check=True,
+                            **get(two))
+        assert (got[0] is None) == (want[0] is None) and (got[0] is None or torch.equal(got[0], want[0]))
+        assert torch.equal(got[1], want[1])
+        assert torch.equal(one["kp"], two["kp"]) and torch.equal(one["vp"], two["vp"])
+    # in place, packed, into the caller's outputs
+    cu = torch.tensor([0, 2, 2, 3], dtype=torch.int32, device=gpu)
+    outs = []
+    for s, check in ((one, False), (two, True)):
+        new, k_out = torch.empty_like(s["lens"]), torch.empty_like(s["k"])
+        r = paged_append(s["k"], s["v"], s["kp"], s["vp"], s["table"], s["lens"], cu, q=s["q"], cos=s["cos"], sin=s["sin"],
+                         q_out=s["q"], k_out=k_out, new_len=new, check=check)
+        assert r[0] is s["q"] and r[1] is new
+        outs.append((s["q"], k_out, new, s["kp"], s["vp"]))
+    assert all(torch.equal(x, y) for x, y in zip(*outs))
+    assert direct_append(one) is not None and direct_append(one, q=None, cos=None, sin=None)[0] is None
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+def test_attention_is_the_checked_call(gpu, dtype):
+    from cast_amd import paged_attention, paged_workspace_bytes
+    s = setup(gpu, dtype)
+    args = (s["q"], s["kp"], s["vp"], s["table"], s["lens"])
+    space = torch.empty(paged_workspace_bytes(3, 10, 16, 8, 2, 64, DT[dtype]), dtype=torch.uint8, device=gpu)
+    for kw in (dict(), dict(softcap=20.0, window=40), dict(kv_split=64), dict(kv_split=-1), dict(sm_scale=0.2),
+               dict(workspace=space)):
+        got = paged_attention(*args, return_lse=True, **kw)
+        want = paged_attention(*args, return_lse=True, check=True, **kw)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        assert torch.equal(paged_attention(*args, **kw), want[0])
+    out = torch.empty_like(s["q"])
+    assert paged_attention(*args, out=out) is out and torch.equal(out, paged_attention(*args, check=True))
+    assert direct_attention(s) is not None
+
+
+def test_what_needs_a_conversion_or_an_error_is_left_alone(gpu):
+    s = setup(gpu)
+    before = s["kp"].clone(), s["vp"].clone()
+    odd = torch.empty(3 * 2 * 64 + 1, dtype=torch.bfloat16, device=gpu)[1:].view(3, 2, 64)      # 2 bytes off
+    common = dict(kp=[s["kp"].cpu(), s["kp"][:0], s["kp"].float(), s["kp"][..., :32], s["kp"].transpose(2, 3), None, 3],
+                  table=[s["table"].cpu(), s["table"].long(), s["table"][:, :0], s["table"][0], [[0]], None],
+                  lens=[s["lens"].cpu(), s["lens"].long(), s["lens"][:2], [1, 2, 3], torch.stack([s["lens"]] * 2, 1)[:, 0]])
+    cases = dict(common, k=[odd, s["k"][:2], s["k"].float(), s["k"].transpose(1, 2), s["k"].cpu()], v=[odd, s["k"][:, :1]],
+                 cu=[[0, 1, 2, 3], s["lens"], torch.zeros(4, dtype=torch.int64, device=gpu)],
+                 q=[s["q"][:2], s["q"][:, :3], s["q"].float(), s["q"][0]],
+                 q_out=[s["q"][:2], s["q"][:1].expand(3, 8, 64), torch.empty_like(s["q"], dtype=torch.float16)],
+                 k_out=[odd, s["k"][:, :1].expand(3, 2, 64)], cos=[s["cos"].double(), s["cos"][:0], s["cos"][:, :30], None],
+                 pos=[[1, 2, 3], s["lens"].long(), s["lens"][:1]], new_len=[s["lens"].long(), s["lens"][:1]])
+    for name, values in cases.items():
+        for i, x in enumerate(values):
+            assert direct_append(s, **{name: x}) is None, (name, i)
+    assert direct_append(s, q=None, q_out=s["q"]) is None
+    assert type(direct_append(s, new_len=s["lens"])) is int                 # the library's own refusal
+    cases = dict(common, q=[s["q"][:2], s["q"][:, :3], s["q"].float(), s["q"][0], s["q"].cpu()], scale=[1, "x"],
+                 cap=[1, -1.0, float("nan"), float("inf")], window=[-1, 1 << 40, 1 << 70, 2.0], split=[-2, 1 << 40, None],
+                 out=[s["q"][:2], s["q"][:1].expand(3, 8, 64), torch.empty_like(s["q"], dtype=torch.float16)],
+                 ws=[torch.empty(64, dtype=torch.uint8, device=gpu), torch.empty(1 << 24, dtype=torch.uint8),
+                     torch.empty(1, dtype=torch.uint8, device=gpu).expand(1 << 24)])
+    for name, values in cases.items():
+        for i, x in enumerate(values):
+            assert direct_attention(s, **{name: x}) is None, (name, i)
+    assert type(direct_attention(s, scale=-1.0)) is int
+    torch.cuda.synchronize()
+    assert torch.equal(s["kp"], before[0]) and torch.equal(s["vp"], before[1])
+
+
+def test_another_stream_and_a_captured_call(gpu):
+    from cast_amd import paged_append, paged_attention
+    s, t = setup(gpu), setup(gpu)
+    new = torch.empty_like(s["lens"])
+    step = lambda x, n, **kw: (paged_append(x["k"], x["v"], x["kp"], x["vp"], x["table"], x["lens"], new_len=n, **kw),
+                               paged_attention(x["q"], x["kp"], x["vp"], x["table"], n, **kw))[1]
+    want = step(t, torch.empty_like(new), check=True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step(s, new)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(s, new)
+    for i in range(3):
+        s["k"].copy_(t["k"].roll(i, 0)), s["q"].mul_(1.5), t["q"].mul_(1.5)
+        s["lens"].add_(1), t["lens"].add_(1)
+        graph.replay()
+        want = step(dict(t, k=t["k"].roll(i, 0)), torch.empty_like(new), check=True)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(s["kp"], t["kp"])

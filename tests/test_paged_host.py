@@ -156,3 +156,12 @@ def test_tree_python_refusals():
     with pytest.raises(ValueError, match="on the GPU"):
         paged_tree_attention(q, pool, pool, torch.zeros((1, 1), dtype=torch.int32), torch.zeros((2, 4, 64)),
                              torch.zeros((2, 4, 64)), [0, 4], [0], [4], torch.zeros(4, dtype=torch.int64))
+
+
+def test_calls_from_tensors_leave_the_host_to_the_wrappers():
+    calls, t = _lib.calls(), torch.zeros((2, 2, 16, 64))
+    assert calls.paged_append(*[t] * 15, 0) is None and calls.paged_append(*[None] * 15, 0) is None
+    assert calls.paged_attention(*[t] * 12, 0) is None and calls.paged_attention(*[3] * 12, 0) is None
+    for f in (calls.paged_append, calls.paged_attention):
+        with pytest.raises(TypeError):
+            f(t)
