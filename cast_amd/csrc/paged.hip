@@ -15,10 +15,10 @@
 //
 // Memory-bound: every row is read once and written once in 16-byte chunks.
 // One thread moves one chunk (one pair of chunks where the two halves of a
-// head rotate into each other); a workgroup's threads belong to one token, so
-// its slot is looked up once, by scalar loads.  Measured: six prompts of up to
-// 4k tokens (8 KV and 32 query heads of 128, bf16) 359 MB in 78 us, 4.6 TB/s; a
-// token each of 8 requests 3.4 us.
+// head rotate into each other); a workgroup's threads belong to one token (or
+// two), so its slot is looked up once, by scalar loads.  Measured: six prompts of
+// up to 4k tokens (8 KV and 32 query heads of 128, bf16) 359 MB in 71 us a call,
+// 5.05 TB/s, a copy's rate; a token each of 8 requests 3.4 us.
 #include "cast_common.hpp"
 
 namespace cast {
@@ -26,6 +26,12 @@ namespace cast {
 constexpr int kPagedLayersPerLaunch = 64;   // four base addresses each in the kernel arguments (2 KiB)
 constexpr int kPagedThreads = 256;
 constexpr int kPathRows = 8;                // workgroups that share a request's accepted rows
+// Rows of a workgroup: two once a row each gives more workgroups than the device
+// holds (8 a CU), so that a second round becomes a second load in flight.  One
+// against two: 512 rows (32 + 8 heads of 128, bf16, 1024 workgroups) 6.3 and 6.8
+// us, 1024 rows 9.5 and 9.3, 4096 26.4 and 25.1; prompts of 13k rows 79 and 71
+// (four: 71 to 72); fp32, 256 rows 6.2 and 6.5, 512 8.8 and 8.6, 4096 45.6 and 42.3.
+constexpr int64_t kOneRowGroups = 2048;
 
 struct PagedAppendArgs {
     const void *q;
@@ -43,7 +49,7 @@ struct PagedAppendArgs {
     int32_t interleaved;
     int32_t units;          // threads per rotated head: a pair of chunks each in the half style
     int32_t tasks;          // threads per token
-    int32_t rows;           // workgroups (x) that move rows; the ones behind check one request each
+    int32_t rows;           // rows to move (path: kPathRows workgroups a request); the workgroups (x) behind theirs check one request each
 };
 
 // The layers' addresses of one launch, of 1 or kPagedLayersPerLaunch layers:
@@ -128,8 +134,16 @@ __device__ __forceinline__ void widen_chunk(u32x4 w, float (&x)[8]) {
         x[2 * i + 1] = E::widen((uint16_t)(bits >> 16));
     }
 }
+// (A float is made of every rotated element first: fp16 has an instruction that
+// rounds a fused product straight to 16 bits, and the compiler takes it in one
+// instance and not in another, where a row should have the same bits in a call
+// of any size.)
 template <typename E>
-__device__ __forceinline__ u32x4 round_chunk(const float (&x)[8]) {
+__device__ __forceinline__ u32x4 round_chunk(float (&x)[8]) {
+    if constexpr (__is_same(E, Fp16)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) asm("" : "+v"(x[i]));
+    }
     return u32x4{E::pack2(x[0], x[1]), E::pack2(x[2], x[3]), E::pack2(x[4], x[5]), E::pack2(x[6], x[7])};
 }
 struct Fp32 {};
@@ -142,7 +156,7 @@ __device__ __forceinline__ void widen_chunk<Fp32>(u32x4 w, float (&x)[8]) {
     }
 }
 template <>
-__device__ __forceinline__ u32x4 round_chunk<Fp32>(const float (&x)[8]) {
+__device__ __forceinline__ u32x4 round_chunk<Fp32>(float (&x)[8]) {
     u32x4 w;
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = __builtin_bit_cast(uint32_t, x[i]);
@@ -164,15 +178,16 @@ __device__ __forceinline__ void load_angles(const float *p, float (&x)[8]) {
     }
 }
 
-template <typename E, int LAYERS>
+template <typename E, int LAYERS, int ROWS>
 __global__ __launch_bounds__(kPagedThreads) void paged_append_kernel(PagedAppendArgs a, PagedLayers<LAYERS> at) {
     constexpr int EPC = __is_same(E, Fp32) ? 4 : 8;   // elements per 16-byte chunk
     const int layer = LAYERS == 1 ? 0 : blockIdx.z;
-    if ((int)blockIdx.x >= a.rows) {
+    const int groups = ROWS == 1 ? a.rows : (int)(((uint32_t)a.rows + ROWS - 1) / ROWS);   // workgroups that move rows
+    if ((int)blockIdx.x >= groups) {
         // ---- one request's check, by its own workgroup: any row that cannot
         // be placed leaves its length as it was
         if (blockIdx.y || layer) return;
-        const int b = blockIdx.x - a.rows;
+        const int b = blockIdx.x - groups;
         const int S = a.seq_len[b];
         int root, n;
         int32_t flags = 0;
@@ -213,13 +228,12 @@ __global__ __launch_bounds__(kPagedThreads) void paged_append_kernel(PagedAppend
     const char *rows = static_cast<const char *>(kind == 0 ? a.q : kind == 1 ? at.k[layer] : at.v[layer]);
     const int64_t row_step = kind == 0 ? a.q_tok : kind == 1 ? a.k_tok : a.v_tok;
     rows += head * (kind == 0 ? a.q_head : kind == 1 ? a.k_head : a.v_head) + chunk * 16;
-    u32x4 x{}, y{};
-    auto load = [&](int64_t src) __attribute__((always_inline)) {
+    auto load = [&](int64_t src, u32x4 &x, u32x4 &y) __attribute__((always_inline)) {
         if (!live) return;
         x = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(rows + src * row_step));   // (read once: 83.5 -> 80 us for 13k tokens)
         if (paired) y = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(rows + src * row_step + far));
     };
-    auto put = [&](const PagedRow &r) __attribute__((always_inline)) {
+    auto put = [&](const PagedRow &r, u32x4 x, u32x4 y) __attribute__((always_inline)) {
         char *to, *also = nullptr;   // also: k_out
         const int64_t src = r.src;
         if (kind == 0) {
@@ -270,28 +284,45 @@ __global__ __launch_bounds__(kPagedThreads) void paged_append_kernel(PagedAppend
         for (int j = blockIdx.x % kPathRows; j < n; j += kPathRows) {
             const PagedRow r = paged_row(a, b, root, j, S);
             if (r.flags || !live) continue;
-            load(r.src);
-            put(r);
+            u32x4 x{}, y{};
+            load(r.src, x, y);
+            put(r, x, y);
         }
         return;
     }
-    // the row is known: its loads run beside the lookups of where it goes
-    const int row = blockIdx.x;
-    load(row);
-    int b = row, root = row, end = row + 1, S;
-    if (a.cu_q) {
-        b = request_of(a, row, root, end, S);
-        // rows behind the last request, offsets that make no sense
-        if (b >= a.batch || root < 0 || root > row || end > a.total) return;
-    } else {
-        S = a.seq_len[b];
+    // the rows are known: their loads run beside the lookups of where they go
+    const int first = blockIdx.x * ROWS;
+    u32x4 x[ROWS], y[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i)
+        if (i == 0 || first + i < a.rows) load(first + i, x[i], y[i]);
+    PagedRow r[ROWS];
+    int b = 0, root = 0, end = first, S = 0;   // the request of rows [root, end)
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        const int row = first + i;
+        r[i].flags = CAST_FLAG_BAD_OFFSETS;
+        if (i && row >= a.rows) continue;
+        if (!a.cu_q) {
+            b = root = row;
+            S = a.seq_len[b];
+        } else if (row >= end) {
+            b = request_of(a, row, root, end, S);
+            // rows behind the last request, offsets that make no sense
+            if (b >= a.batch || root < 0 || root > row || end > a.total) {
+                end = row;
+                continue;
+            }
+        }
+        r[i] = paged_row(a, b, root, row - root, S);
     }
-    const PagedRow r = paged_row(a, b, root, row - root, S);
-    if (r.flags || !live) return;
-    put(r);
+    if (!live) return;
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i)
+        if (!r[i].flags) put(r[i], x[i], y[i]);
 }
 
-template <int LAYERS>
+template <int LAYERS, int ROWS>
 static int launch_append(const PagedAppendArgs &a, const void *const *k, const void *const *v, void *const *k_pages,
                          void *const *v_pages, int32_t n, int32_t dtype, dim3 grid, hipStream_t st) {
     PagedLayers<LAYERS> at{};
@@ -301,9 +332,9 @@ static int launch_append(const PagedAppendArgs &a, const void *const *k, const v
         at.k_pages[l] = k_pages[l];
         at.v_pages[l] = v_pages[l];
     }
-    if (dtype == CAST_BF16) paged_append_kernel<Bf16, LAYERS><<<grid, kPagedThreads, 0, st>>>(a, at);
-    else if (dtype == CAST_FP16) paged_append_kernel<Fp16, LAYERS><<<grid, kPagedThreads, 0, st>>>(a, at);
-    else paged_append_kernel<Fp32, LAYERS><<<grid, kPagedThreads, 0, st>>>(a, at);
+    if (dtype == CAST_BF16) paged_append_kernel<Bf16, LAYERS, ROWS><<<grid, kPagedThreads, 0, st>>>(a, at);
+    else if (dtype == CAST_FP16) paged_append_kernel<Fp16, LAYERS, ROWS><<<grid, kPagedThreads, 0, st>>>(a, at);
+    else paged_append_kernel<Fp32, LAYERS, ROWS><<<grid, kPagedThreads, 0, st>>>(a, at);
     return hipGetLastError() == hipSuccess ? CAST_OK : CAST_ERR_HIP;
 }
 
@@ -409,12 +440,12 @@ extern "C" int cast_paged_append(const void *const *k, const void *const *v, voi
         const int32_t n = layers - l0 < kPagedLayersPerLaunch ? layers - l0 : kPagedLayersPerLaunch;
         const bool checks = l0 == 0 && (new_len || status);
         a.new_len = checks ? new_len : nullptr;
-        const dim3 grid((unsigned)(a.rows + (checks ? batch : 0)), (unsigned)slices, (unsigned)n);
+        const bool two = n == 1 && !path && rows * slices >= kOneRowGroups;
+        const dim3 grid((unsigned)((two ? (rows + 1) / 2 : rows) + (checks ? batch : 0)), (unsigned)slices, (unsigned)n);
         if (grid.x == 0) continue;
         hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-        const int rc = n == 1 ? launch_append<1>(a, k + l0, v + l0, k_pages + l0, v_pages + l0, 1, dtype, grid, st)
-                              : launch_append<kPagedLayersPerLaunch>(a, k + l0, v + l0, k_pages + l0, v_pages + l0, n, dtype,
-                                                                     grid, st);
+        auto *const run = n > 1 ? launch_append<kPagedLayersPerLaunch, 1> : two ? launch_append<1, 2> : launch_append<1, 1>;
+        const int rc = run(a, k + l0, v + l0, k_pages + l0, v_pages + l0, n, dtype, grid, st);
         if (rc != CAST_OK) return rc;
     }
     return CAST_OK;

@@ -530,3 +530,60 @@ def test_empty_tables_strided_workspaces_and_sizes_past_31_bits(gpu):
     assert torch.equal(paged_attention(q, kp, vp, table, lens, window=(1 << 32) + 5, kv_split=-1), ref)
     assert torch.equal(paged_attention(q, kp, vp, table, lens, kv_split=(1 << 32) + 128), ref)
     assert torch.equal(paged_attention(q, kp, vp, table, lens, kv_split=-(1 << 32) + 128), ref)
+
+
+@pytest.mark.parametrize("dtype,D,inter", [("bf16", 64, False), ("fp16", 128, True), ("fp32", 40, False)])
+def test_two_rows_a_workgroup_are_the_rows_one_by_one(gpu, dtype, D, inter):
+    # a call of more rows than the device holds workgroups, an odd number and some behind the last request, against
+    # calls of a few requests each: the same bits, in packed and in one-row-each form
+    from cast_amd import paged_append
+    rng, dt = np.random.default_rng(7), DT[dtype]
+    B, ps = 400, 4
+    new = rng.integers(0, 13, size=B)
+    new[5], new[77], new[78] = 1, 0, 0
+    new[-1] += 1 - new.sum() % 2                       # odd
+    seq = rng.integers(0, 9, size=B)
+    cu = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    total, tail = int(cu[-1]), 2
+    assert total % 2 and total >= 2048
+    g = torch.Generator().manual_seed(3)
+    k, v, q = (torch.randn((total + tail, h, D), generator=g).to(dt).to(gpu) for h in (1, 1, 2))
+    width = int(-(-(seq + new).max() // ps))
+    table = torch.randperm(B * width, generator=g).view(B, width).int()
+    table[9] = -1                                      # this request has no pages
+    new[9] or pytest.fail("the request without pages needs rows")
+    table = table.to(gpu)
+    cos, sin = (x.to(gpu) for x in tables(64, 32, gpu))
+    start = torch.from_numpy(seq.astype(np.int32)).to(gpu)
+
+    def fresh():
+        return [torch.full((B * width, 1, ps, D), 5.0, dtype=dt, device=gpu) for _ in range(2)]
+
+    def call(pools, lo, hi, rows, offsets):
+        q_out = torch.full_like(q[rows], 7.0)
+        _, n = paged_append(k[rows], v[rows], *pools, table[lo:hi], start[lo:hi], offsets, q=q[rows], q_out=q_out, cos=cos,
+                            sin=sin, interleaved=inter)
+        return q_out, n
+
+    big, small = fresh(), fresh()
+    q_big, n_big = call(big, 0, B, slice(0, total + tail), torch.from_numpy(cu).to(gpu))
+    parts = []
+    for lo in range(0, B, 50):
+        rows = slice(int(cu[lo]), int(cu[lo + 50]))
+        parts.append(call(small, lo, lo + 50, rows, torch.from_numpy(cu[lo:lo + 51] - cu[lo]).to(gpu)))
+    assert torch.equal(q_big[:total], torch.cat([x for x, _ in parts])) and (q_big[total:] == 7).all()
+    assert torch.equal(n_big, torch.cat([n for _, n in parts])) and n_big[9] == seq[9]
+    assert all(torch.equal(x, y) for x, y in zip(big, small))
+    assert (q_big[int(cu[9]):int(cu[10])] == 7).all()
+    # one row each, 2401 requests that take turns at the tables' rows
+    many = torch.arange(2401, device=gpu) % B
+    pools, again = fresh(), fresh()
+    lens = (torch.arange(2401, device=gpu) // B).int()             # (rows of one request go to different slots)
+    rows = torch.arange(2401, device=gpu) % total
+    ks, vs, t = k[rows], v[rows], table[many]
+    _, n = paged_append(ks, vs, *pools, t, lens, cos=cos, sin=sin, interleaved=inter)
+    for lo in range(0, 2401, 343):
+        _, m = paged_append(ks[lo:lo + 343], vs[lo:lo + 343], *again, t[lo:lo + 343], lens[lo:lo + 343], cos=cos, sin=sin,
+                            interleaved=inter)
+        assert torch.equal(n[lo:lo + 343], m)
+    assert all(torch.equal(x, y) for x, y in zip(pools, again))
