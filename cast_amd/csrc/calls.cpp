@@ -3,8 +3,9 @@
 //
 // A decode step makes two of these calls a layer, and its kernels take 3 to 12 us
 // where few requests run; with some ten tensors checked and 50 arguments
-// converted in Python a call took 17.5 us of the host, here it takes 6.0
-// (append) and 10.0 (attention; 8 of them two launches).  Each function repeats the conditions
+// converted in Python a call took 17.5 us of the host (the tree attention 22.8),
+// here it takes 6 (append) and 9 to 10 (attention, 6.5 of them two launches).
+// Each function repeats the conditions
 // of its wrapper in cast_amd/paged.py and either makes the call, or returns
 // None: the wrapper then converts what can be converted and words the error
 // for what cannot.  The result is the wrapper's, or the cast_status of a call
@@ -75,7 +76,7 @@ struct Pools {
         }
         ok = (low * esz & 15) == 0 && aligned(k) && aligned(v);
     }
-    // [rows, heads, D] of the pools' type, as it lies
+    // [n, heads, D] of the pools' type, as it lies
     bool rows(const at::Tensor &t, int64_t n, int64_t heads) const {
         return t.dim() == 3 && t.scalar_type() == dtype && t.is_cuda() && t.device().index() == index && t.size(0) == n &&
                t.size(1) == heads && t.size(2) == D && t.stride(2) == 1 && ((t.stride(0) | t.stride(1)) * esz & 15) == 0 &&
@@ -243,9 +244,81 @@ PyObject *paged_attention(PyObject *, PyObject *const *o, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// paged_tree_attention(q, k_pages, v_pages, page_table, k_pack, v_pack, cu_q,
+//                      prefix_len, pack_len, ancestor_mask, sm_scale, total_kv,
+//                      return_lse, kv_split, out, workspace, stream)
+PyObject *paged_tree_attention(PyObject *, PyObject *const *o, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 17) {
+        PyErr_SetString(PyExc_TypeError, "paged_tree_attention takes 17 arguments");
+        return nullptr;
+    }
+    const Arg q(o[0]), kp(o[1]), vp(o[2]), table(o[3]), kn(o[4]), vn(o[5]), cu(o[6]), pre(o[7]), pack(o[8]), mask(o[9]),
+        out(o[14]), ws(o[15]);
+    for (const Arg *a : {&q, &kp, &vp, &table, &kn, &vn, &cu, &pre, &pack, &mask, &out, &ws})
+        if (!a->ok) Py_RETURN_NONE;
+    if (!q || !kp || !vp || !table || !kn || !vn || !cu || !pre || !pack || !mask) Py_RETURN_NONE;
+    const Pools pools(*kp, *vp);
+    if (!pools.ok || !pools.table(*table) || q->dim() != 3) Py_RETURN_NONE;
+    const int64_t B = table->size(0), max_pages = table->size(1), total_q = q->size(0), H_q = q->size(1);
+    if (!total_q || total_q > kInt32 || !H_q || H_q % pools.H_kv || H_q > kInt32 || !pools.rows(*q, total_q, H_q)) Py_RETURN_NONE;
+    if (pools.page_size % 64 && max_pages > 1) Py_RETURN_NONE;
+    for (const Arg *a : {&kn, &vn})
+        if (!pools.rows(**a, pools.H_kv, total_q)) Py_RETURN_NONE;   // (head-major)
+    if (!pools.ints(*cu, B + 1) || !pools.ints(*pre, B) || !pools.ints(*pack, B)) Py_RETURN_NONE;
+    if (mask->scalar_type() != at::kLong || !mask->is_cuda() || mask->device().index() != pools.index ||
+        !mask->is_contiguous() || mask->dim() < 1 || mask->dim() > 2 || mask->size(0) != total_q)
+        Py_RETURN_NONE;
+    const int64_t words = mask->dim() == 1 ? 1 : mask->size(1);
+    if (words < 1 || words > 2) Py_RETURN_NONE;
+    if (out && !pools.output(*out, total_q, H_q)) Py_RETURN_NONE;
+    if ((o[10] != Py_None && !PyFloat_Check(o[10])) || (o[11] != Py_None && !PyLong_Check(o[11])) || !PyLong_Check(o[13]))
+        Py_RETURN_NONE;
+    const double scale = o[10] == Py_None ? 1.0 / std::sqrt((double)pools.D) : PyFloat_AS_DOUBLE(o[10]);
+    int past = 0, past2;
+    if (o[11] == Py_None && max_pages * pools.page_size > kInt32) Py_RETURN_NONE;
+    const int64_t total_kv =
+        o[11] == Py_None ? B * max_pages * pools.page_size + total_q : PyLong_AsLongLongAndOverflow(o[11], &past);
+    const long long split = PyLong_AsLongLongAndOverflow(o[13], &past2);
+    if (past || past2 || total_kv < 0 || total_kv > kInt32 || split < -kInt32 || split > kInt32) Py_RETURN_NONE;
+    const int lse_too = PyObject_IsTrue(o[12]);
+    if (lse_too < 0) return nullptr;
+    const auto stream = reinterpret_cast<cast_stream_t>(PyLong_AsVoidPtr(o[16]));
+    if (PyErr_Occurred()) return nullptr;
+    const size_t need =
+        cast_tree_attn_paged_workspace_size((int32_t)B, (int32_t)total_q, (int32_t)total_kv, (int32_t)H_q, (int32_t)pools.H_kv,
+                                            (int32_t)pools.D, pools.code, (int32_t)split);
+    if (ws && (!ws->is_cuda() || ws->device().index() != pools.index || !ws->is_contiguous() || ws->nbytes() < need))
+        Py_RETURN_NONE;
+
+    at::Tensor made, lse, made_ws;
+    const at::Tensor *to = out.t;
+    if (!to) to = &(made = at::empty({total_q, H_q, pools.D}, q->options()));
+    if (lse_too) lse = at::empty({total_q, H_q}, q->options().dtype(at::kFloat));
+    void *space = ws ? ws->data_ptr() : (made_ws = at::empty({(int64_t)need}, q->options().dtype(at::kByte))).data_ptr();
+    const int64_t *sk = kp->strides().data(), *sv = vp->strides().data();
+    int st;
+    Py_BEGIN_ALLOW_THREADS;
+    st = cast_tree_attn_paged_fwd(
+        q->data_ptr(), kp->data_ptr(), vp->data_ptr(), at_of<int32_t>(table), table->stride(0), (int32_t)max_pages,
+        (int32_t)pools.pages, (int32_t)pools.page_size, kn->data_ptr(), vn->data_ptr(), to->data_ptr(),
+        lse_too ? static_cast<float *>(lse.data_ptr()) : nullptr, at_of<int32_t>(cu), at_of<int32_t>(pre), at_of<int32_t>(pack),
+        static_cast<const uint64_t *>(mask->data_ptr()), (int32_t)words, (int32_t)B, (int32_t)total_q, (int32_t)total_kv,
+        (int32_t)H_q, (int32_t)pools.H_kv, (int32_t)pools.D, q->stride(0), q->stride(1), sk[0], sk[1], sk[2], sv[0], sv[1],
+        sv[2], kn->stride(1), kn->stride(0), vn->stride(1), vn->stride(0), to->stride(0), to->stride(1), pools.code,
+        (float)scale, (int32_t)split, space, need, nullptr, stream);
+    Py_END_ALLOW_THREADS;
+    if (st) return PyLong_FromLong(st);
+    PyObject *r = made.defined() ? THPVariable_Wrap(made) : Py_NewRef(o[14]);
+    return lse_too ? pair(r, THPVariable_Wrap(lse)) : r;
+    END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
     {"paged_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(paged_append)), METH_FASTCALL, nullptr},
     {"paged_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(paged_attention)), METH_FASTCALL, nullptr},
+    {"paged_tree_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(paged_tree_attention)), METH_FASTCALL,
+     nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

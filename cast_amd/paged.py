@@ -337,8 +337,17 @@ def paged_tree_attention(q, k_pages, v_pages, page_table, k_pack, v_pack, cu_q, 
     request whose prefix names a page outside the pool is rejected like one with
     inconsistent lengths: zeros with lse = -inf, and ``check=True`` raises.
     """
-    lib = _lib.load()
     kv_split = max(-_INT32, min(operator.index(kv_split), _INT32))
+    if not check and k_pages.is_cuda:
+        done = _lib.calls().paged_tree_attention(q, k_pages, v_pages, page_table, k_pack, v_pack, cu_q, prefix_len, pack_len,
+                                                 ancestor_mask, sm_scale, total_kv, return_lse, kv_split, out, workspace,
+                                                 _lib.stream_of(k_pages))
+        if type(done) is int:
+            _lib.check(done, "cast_tree_attn_paged_fwd")
+        if done is not None:
+            return done
+    # (a status to read, a copy to make, or something to refuse)
+    lib = _lib.load()
     pools = _Pools(k_pages, v_pages, "paged_tree_attention")
     H_kv, D, dev = pools.H_kv, pools.D, pools.device
     if pools.n_pages == 0:

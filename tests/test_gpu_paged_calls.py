@@ -138,3 +138,65 @@ def test_another_stream_and_a_captured_call(gpu):
         want = step(dict(t, k=t["k"].roll(i, 0)), torch.empty_like(new), check=True)
         torch.cuda.synchronize()
         assert torch.equal(got, want) and torch.equal(s["kp"], t["kp"])
+
+
+def tree_setup(gpu, dtype="bf16", B=3, Hq=8, Hkv=2, D=64, ps=64, pages=20, width=5, seed=0):
+    s = setup(gpu, dtype, B, Hq, Hkv, D, ps, pages, width, seed)
+    g = torch.Generator().manual_seed(seed + 1)
+    pack = torch.tensor([1, 20, 7][:B])
+    total = int(pack.sum())
+    rnd = lambda *shape: torch.randn(shape, generator=g).to(DT[dtype]).to(gpu)
+    ints = lambda x: torch.as_tensor(x).int().to(gpu)
+    words = torch.cat([(1 << torch.arange(1, int(p) + 1)) - 1 for p in pack])      # chains
+    return dict(q=rnd(total, Hq, D), kp=s["kp"], vp=s["vp"], table=s["table"], kn=rnd(Hkv, total, D), vn=rnd(Hkv, total, D),
+                cu=ints([0, *pack.cumsum(0).tolist()]), pre=ints([200, 0, 131]), pack=ints(pack), mask=words.to(gpu))
+
+
+def direct_tree(s, **over):
+    from cast_amd import _lib
+    a = dict(s, scale=None, total_kv=None, lse=False, split=0, out=None, ws=None)
+    a.update(over)
+    return _lib.calls().paged_tree_attention(*a.values(), stream(s["kp"]))
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+def test_tree_attention_is_the_checked_call(gpu, dtype):
+    from cast_amd import paged_tree_attention
+    from cast_amd.paged import paged_tree_workspace_bytes
+    s = tree_setup(gpu, dtype)
+    two = torch.stack([s["mask"], torch.zeros_like(s["mask"])], 1)
+    space = torch.empty(paged_tree_workspace_bytes(s["q"], s["kp"], s["table"], 400), dtype=torch.uint8, device=gpu)
+    cases = (dict(), dict(total_kv=400), dict(total_kv=400, workspace=space), dict(kv_split=64), dict(sm_scale=0.2),
+             dict(kv_split=-1), dict(kv_split=-2), dict(ancestor_mask=two))
+    for kw in cases:
+        args = dict(zip(("q", "k_pages", "v_pages", "page_table", "k_pack", "v_pack", "cu_q", "prefix_len", "pack_len",
+                         "ancestor_mask"), s.values()))
+        args.update(kw)
+        got = paged_tree_attention(**args, return_lse=True)
+        want = paged_tree_attention(**args, return_lse=True, check=True)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), kw
+        assert torch.equal(paged_tree_attention(**args), want[0])
+    # (packs as a forward hands them over: token-major, seen head-major)
+    kn, vn = (s[x].transpose(0, 1).contiguous().transpose(0, 1) for x in ("kn", "vn"))
+    out = torch.empty_like(s["q"])
+    assert direct_tree(s, kn=kn, vn=vn, out=out) is out
+    assert torch.equal(out, direct_tree(s))
+
+
+def test_tree_calls_that_need_a_conversion_or_an_error_are_left_alone(gpu):
+    s = tree_setup(gpu)
+    cases = dict(q=[s["q"][:3], s["q"][:, :3], s["q"].float(), s["q"][0]],
+                 kp=[s["kp"].cpu(), s["kp"][:0], s["kp"].float(), s["kp"][:, :, :48], s["kp"][..., :32], None],
+                 table=[s["table"].cpu(), s["table"].long(), s["table"][:2], [[0]]],
+                 kn=[s["kn"].transpose(0, 1), s["kn"][:, :4], s["kn"].float(), s["kn"].cpu()], vn=[s["vn"][:1]],
+                 cu=[s["cu"][:3], s["cu"].long(), s["cu"].cpu(), [0, 1, 21, 28]], pre=[s["pre"].cpu(), [200, 0, 131]],
+                 pack=[s["pack"][:2], s["pack"].long()], mask=[s["mask"].int(), s["mask"][:5], s["mask"].cpu(), s["mask"][:, None, None],
+                                                               s["mask"][:, None].expand(-1, 3), s["mask"][:, None].expand(-1, 2)],
+                 scale=[1, "x"], total_kv=[-1, 1 << 31, 1 << 70, 2.0], split=[None, 1 << 40],
+                 out=[s["q"][:3], s["q"][:1].expand(28, 8, 64)],
+                 ws=[torch.empty(64, dtype=torch.uint8, device=gpu), torch.empty(1 << 22, dtype=torch.uint8),
+                     torch.empty(1, dtype=torch.uint8, device=gpu).expand(1 << 24)])
+    for name, values in cases.items():
+        for i, x in enumerate(values):
+            assert direct_tree(s, **{name: x}) is None, (name, i)
+    assert type(direct_tree(s, scale=-1.0)) is int

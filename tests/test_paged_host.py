@@ -162,6 +162,7 @@ def test_calls_from_tensors_leave_the_host_to_the_wrappers():
     calls, t = _lib.calls(), torch.zeros((2, 2, 16, 64))
     assert calls.paged_append(*[t] * 15, 0) is None and calls.paged_append(*[None] * 15, 0) is None
     assert calls.paged_attention(*[t] * 12, 0) is None and calls.paged_attention(*[3] * 12, 0) is None
-    for f in (calls.paged_append, calls.paged_attention):
+    assert calls.paged_tree_attention(*[t] * 16, 0) is None and calls.paged_tree_attention(*[3] * 16, 0) is None
+    for f in (calls.paged_append, calls.paged_attention, calls.paged_tree_attention):
         with pytest.raises(TypeError):
             f(t)
