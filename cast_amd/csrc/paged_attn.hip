@@ -54,7 +54,7 @@ constexpr float kPLn2 = 0.69314718055994530942f;
 constexpr float kPLog2e = 1.44269504088896340736f;
 constexpr int kPWaves = 4;
 // What a piece costs beside its tiles, in tiles of 32 KB (head dim 64) and of
-// 64 KB and more: 200 requests of up to 1k keys at D = 64, fp16, 43.3, 36.5, 35.2
+// 64 KB and more (measured before units that cannot be long were left whole): 200 requests of up to 1k keys at D = 64, fp16, 43.3, 36.5, 35.2
 // and 35.9 us for 0 to 3; 64 of 300 to 8k at D = 128, bf16, 219.5, 222, 225, 230.
 constexpr int piece_cost(int D) { return D == 64 ? 2 : 1; }
 constexpr int kLensLds = 1024;           // batches whose lengths a workgroup keeps in LDS for its schedule
@@ -64,7 +64,7 @@ constexpr int kMinTiles = 1;
 // Tiles a workgroup should have before a CU gets a second one, where units are
 // fewer than CUs: one request of 32k keys 24.1 + 4.0 us (attention, join) on 256
 // workgroups of 8 tiles, 24.8 + 5.0 on 512 of 4.  (Units of their own are better
-// spread: 200 requests of up to 1k keys, 4 KV heads, 35 us on 768, 37.6 on 440.)
+// spread: 200 requests of up to 1k keys, 4 KV heads, scheduled: 35 us on 768, 37.6 on 440.)
 constexpr int kFewTiles = 8;
 
 struct PagedAttnArgs {
@@ -923,22 +923,44 @@ static PagedDevice paged_slots(const PagedKernel &k) {
     return d;
 }
 
+// Whether units of at most `bytes` of K and V get a workgroup each and no
+// pieces, which saves the join's launch (4 to 5 us) and the schedule.  Split
+// against whole, us, units of a batch's longest request (or of lengths spread
+// evenly below it), 64-key pages, 4 query heads a KV head:
+//   bf16, D 128, 256 KB:  32 units 13.2 and 11.0, 256 22.5 and 16.5, 1024 50.2 and 45.4
+//   the same, 512 KB:     32 units 13.9 and 16.2, 128 21.4 and 18.4 (17.3 and 17.0), 1024 88.1 and 84.1 (60.1 and 53.1)
+//   1 MB:                 128 units 30.9 and 29.3 (26.3 and 27.2), 1024 168 and 165 (98.7 and 98.3)
+//   bf16, D 64, 256 KB:   32 units 11.8 and 11.9, 128 15.1 and 12.2, 1024 54.3 and 43.8
+//   fp32, D 128, 512 KB:  32 units 13.8 and 19.0, 128 21.3 and 20.5 (18.3 and 19.7), 1024 91.4 and 86.8
+//   bf16, D 256, 512 KB:  128 units 24.2 and 22.7 (20.8 and 21.3), 512 54.3 and 52.8, 1024 98.1 and 103.9 (79.2 and 74.1)
+// Pages whose keys are looked up one by one (`any`) take a tile twice as long:
+//   bf16, D 128, 256 KB:  32 units 13.4 and 15.1, 128 17.2 and 16.1 (16.4 and 15.4), 1024 69.9 and 64.0
+//   the same, 512 KB:     128 units 22.6 and 26.4 (19.1 and 25.1)
+// 1 MB would pay from 256 units of like lengths on, but there one long request
+// among short ones would keep all waiting.
+static bool paged_whole(int64_t bytes, int64_t units, bool any, int cus) {
+    return (any ? 2 * bytes : bytes) <= (2 * units >= cus ? 512 << 10 : 256 << 10);
+}
+
 struct PagedPlan {
     int32_t wgs, least, cut, cus;   // as PagedAttnArgs
     bool fits;            // tile indices fit 31 bits for any lengths
 };
 static PagedPlan paged_plan(int32_t batch, int32_t max_pages, int32_t page_size, int32_t Hq, int32_t Hkv, int32_t D,
                             int32_t window, int32_t dtype, int32_t kv_split) {
-    const PagedKernel k = paged_kernel(dtype, D, paged_any(page_size, max_pages));
+    const bool any = paged_any(page_size, max_pages);
+    const PagedKernel k = paged_kernel(dtype, D, any);
     const int64_t units = (int64_t)batch * Hkv * ((Hq / Hkv + 15) / 16);
     int64_t keys = (int64_t)max_pages * page_size;
     if (window > 0 && window < keys) keys = (int64_t)window + k.tile - 1;   // (a window may start inside a tile)
     const int64_t tiles = (keys + k.tile - 1) / k.tile;
     const int64_t least = kv_split > 0 ? ((int64_t)kv_split + k.tile - 1) / k.tile : kMinTiles;
-    if (kv_split < 0 || tiles <= least) return {units > INT_MAX ? 0 : (int32_t)units, 0, 0, 0, units <= INT_MAX};
+    const PagedDevice d = paged_slots(k);
+    const bool whole = kv_split < 0 || tiles <= least ||
+                       (kv_split == 0 && paged_whole(tiles * k.tile * D * (dtype == CAST_FP32 ? 8 : 4), units, any, d.cus));
+    if (whole) return {units > INT_MAX ? 0 : (int32_t)units, 0, 0, 0, units <= INT_MAX};
     if (units > INT_MAX / (tiles + piece_cost(64))) return {0, 0, 0, 0, false};
     const int64_t most = units * ((tiles + least - 1) / least);
-    const PagedDevice d = paged_slots(k);
     const int64_t wgs = kv_split > 0 ? most : std::min<int64_t>(most, d.slots);
     return {(int32_t)wgs, (int32_t)least, kv_split > 0, d.cus, true};
 }

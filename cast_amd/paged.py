@@ -244,7 +244,7 @@ def paged_attention(q, k_pages, v_pages, page_table, seq_len, sm_scale=None, *, 
     positive; with ``window > 0`` only the last ``window`` slots are seen.
     ``return_lse`` also returns their natural-log log-sum-exp [B, H_q] (fp32).
     ``kv_split``: keys per split of a request (0: chosen on the device from the
-    lengths; negative: no split).  ``workspace``: uint8 device tensor of at
+    lengths, none where table rows or the window are short; negative: none).  ``workspace``: uint8 device tensor of at
     least ``paged_workspace_bytes(...)``; one is allocated when missing or too
     small.  Calls that share a workspace must not overlap.
 

@@ -403,8 +403,8 @@ int cast_build_trees_uniform(const int64_t *top_idx, const void *top_lp, int32_t
  * Rotation, q and k_out take one layer and no path.  A row whose slot, page
  * id or position is out of range is skipped whole (its pages, q_out and
  * k_out rows keep what they held); *status gets CAST_FLAG_BAD_OFFSETS,
- * _BAD_PAGE or _BAD_POSITION.  Where cu_q decreases, every new_len is seq_len.  Two rows that the tables send to one slot
- * leave either's elements.
+ * _BAD_PAGE or _BAD_POSITION.  Where cu_q decreases, every new_len is seq_len.
+ * Two rows that the tables send to one slot leave either's elements.
  * ------------------------------------------------------------------- */
 int cast_paged_append(const void *const *k, const void *const *v, void *const *k_pages,
                       void *const *v_pages, int32_t layers, const int32_t *page_table,
@@ -434,8 +434,9 @@ int cast_paged_append(const void *const *k, const void *const *v, void *const *k
  *            front of the window are not looked up
  *   head_dim any multiple of 8 up to 256; dtypes CAST_BF16, _FP16, _FP32
  *   kv_split keys per split (rounded up to key tiles of 128, fp32 64); 0: an
- *            even share of the workgroups the device holds, from the lengths;
- *            negative: one split
+ *            even share of the workgroups the device holds, from the lengths,
+ *            or one split where table rows (or the window) are short; negative:
+ *            one split
  *   workspace  cast_paged_attn_workspace_size(...) bytes, 256-byte aligned
  *            (may be NULL when that is 0); calls sharing one must not overlap
  * A request whose seq_len is outside [0, max_pages * page_size]

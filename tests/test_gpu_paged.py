@@ -587,3 +587,35 @@ def test_two_rows_a_workgroup_are_the_rows_one_by_one(gpu, dtype, D, inter):
                             interleaved=inter)
         assert torch.equal(n[lo:lo + 343], m)
     assert all(torch.equal(x, y) for x, y in zip(pools, again))
+
+
+WIDE = [c for c in CASES if c[9] == 0 and c[7] == 0] + [
+    # dtype, Hq, Hkv, D, page size, layout, lengths (window, softcap, kv_split)
+    ("bf16", 8, 2, 128, 64, "hnd", [3000, 0, 1, 128, 129, 2048], 0, 0.0, 0),
+    ("fp32", 4, 2, 96, 24, "nhd", [1200, 64, 0, 65], 0, 10.0, 0),
+    ("fp16", 8, 4, 64, 16, "hnd", [int(x) for x in np.random.default_rng(9).integers(0, 500, 90)], 0, 0.0, 0),
+    ("bf16", 4, 4, 256, 32, "hnd", [int(x) for x in np.random.default_rng(8).integers(0, 400, 70)], 0, 0.0, 0),
+    ("bf16", 8, 8, 64, 16, "nhd", [int(x) for x in np.random.default_rng(7).integers(0, 300, 110)], 0, 0.0, 0),   # more units than workgroups
+]
+
+
+@pytest.mark.parametrize("case", WIDE, ids=lambda c: "-".join(str(x) for x in c[:5]) + f"-b{len(c[6])}")
+def test_wide_tables_take_the_schedule_and_narrow_ones_do_not(gpu, case):
+    # a unit that may be long is scheduled from the lengths and joined, one that cannot gets a workgroup: both
+    # against 64 bits, whatever the tables hold behind the last page
+    from cast_amd import paged_attention, paged_workspace_bytes
+    dtype, Hq, Hkv, D, ps, layout, lens, _, softcap, _ = case
+    print("case wide", case[:6], flush=True)
+    kp, vp, table, g = make_cache(gpu, lens, Hkv, D, ps, dtype, layout, seed=len(lens) + D)
+    q = torch.randn((len(lens), Hq, D), generator=g).to(DT[dtype])
+    ref = OP.attention(q, kp, vp, table, lens, softcap=softcap)
+    dev = lambda x: x.to(gpu)
+    kd = dev(kp) if layout == "hnd" else dev(kp.transpose(1, 2).contiguous()).transpose(1, 2)
+    vd = dev(vp) if layout == "hnd" else dev(vp.transpose(1, 2).contiguous()).transpose(1, 2)
+    L = torch.tensor(lens, dtype=torch.int32, device=gpu)
+    wide = torch.full((len(lens), (1 << 20) // ps), -9, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    assert paged_workspace_bytes(len(lens), wide.shape[1], ps, Hq, Hkv, D, DT[dtype]) > 0
+    for t in (table, wide):
+        out, lse = paged_attention(dev(q), kd, vd, dev(t), L, softcap=softcap, return_lse=True, check=True)
+        check_attention(out, lse, ref, DT[dtype], max(lens), D)

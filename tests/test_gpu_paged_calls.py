@@ -109,7 +109,7 @@ def test_what_needs_a_conversion_or_an_error_is_left_alone(gpu):
                      torch.empty(1, dtype=torch.uint8, device=gpu).expand(1 << 24)])
     for name, values in cases.items():
         for i, x in enumerate(values):
-            assert direct_attention(s, **{name: x}) is None, (name, i)
+            assert direct_attention(s, **{"split": 64, name: x}) is None, (name, i)
     assert type(direct_attention(s, scale=-1.0)) is int
     torch.cuda.synchronize()
     assert torch.equal(s["kp"], before[0]) and torch.equal(s["vp"], before[1])
