@@ -596,6 +596,7 @@ WIDE = [c for c in CASES if c[9] == 0 and c[7] == 0] + [
     ("fp16", 8, 4, 64, 16, "hnd", [int(x) for x in np.random.default_rng(9).integers(0, 500, 90)], 0, 0.0, 0),
     ("bf16", 4, 4, 256, 32, "hnd", [int(x) for x in np.random.default_rng(8).integers(0, 400, 70)], 0, 0.0, 0),
     ("bf16", 8, 8, 64, 16, "nhd", [int(x) for x in np.random.default_rng(7).integers(0, 300, 110)], 0, 0.0, 0),   # more units than workgroups
+    ("fp16", 2, 1, 64, 16, "hnd", [int(x) for x in np.random.default_rng(6).integers(0, 60, 1500)], 0, 0.0, 0),   # lengths past LDS
 ]
 
 

@@ -200,3 +200,52 @@ def test_tree_calls_that_need_a_conversion_or_an_error_are_left_alone(gpu):
         for i, x in enumerate(values):
             assert direct_tree(s, **{name: x}) is None, (name, i)
     assert type(direct_tree(s, scale=-1.0)) is int
+
+
+def test_shared_pages_cut_tables_and_output_over_the_queries(gpu):
+    # two requests that share their pages, a table that is some columns of a wider one, results over q: the same bits
+    from cast_amd import paged_attention
+    for width, split in ((10, 0), (10, 64), (200, 0)):
+        s = setup(gpu, pages=40, width=10)
+        table = torch.zeros((3, width + 3), dtype=torch.int32, device=gpu)
+        table[:, :10] = s["table"]
+        table[1, :10] = table[0, :10]
+        lens = torch.tensor([130, 130, 77], dtype=torch.int32, device=gpu)
+        q = s["q"].clone()
+        q[1] = q[0]
+        want = paged_attention(q, s["kp"], s["vp"], table[:, :width].contiguous(), lens, kv_split=split)
+        assert torch.equal(want[0], want[1])
+        assert torch.equal(paged_attention(q, s["kp"], s["vp"], table[:, :width], lens, kv_split=split), want)
+        assert paged_attention(q, s["kp"], s["vp"], table[:, :width], lens, kv_split=split, out=q) is q
+        assert torch.equal(q, want)
+
+
+def test_captured_tree_calls_replay_with_new_lengths_and_pages(gpu):
+    # two captured calls that share a workspace; lengths, tables and inputs change in place between replays
+    from cast_amd import paged_tree_attention
+    from cast_amd.paged import paged_tree_workspace_bytes
+    sets = [tree_setup(gpu, seed=i) for i in range(2)]
+    space = torch.empty(paged_tree_workspace_bytes(sets[0]["q"], sets[0]["kp"], sets[0]["table"], 1000, 64), dtype=torch.uint8,
+                        device=gpu)
+    call = lambda s, **kw: paged_tree_attention(*s.values(), total_kv=1000, kv_split=64, **kw)
+    for s in sets:
+        call(s, workspace=space)
+    outs, graphs = [torch.empty_like(s["q"]) for s in sets], [torch.cuda.CUDAGraph() for _ in sets]
+    for i, s in enumerate(sets):
+        with torch.cuda.graph(graphs[i]):
+            call(s, out=outs[i], workspace=space)
+    for step in range(4):
+        for i, s in enumerate(sets):
+            s["pre"].copy_(torch.tensor([200 + step, 64 * step, 131 - 3 * step], dtype=torch.int32))
+            s["table"].copy_(s["table"].roll(1, 1))
+            if step == 2:
+                s["table"][2, 0] = -1                       # (rejected in this step alone)
+            s["q"].mul_(-1.25)
+            want = call(s)
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            assert torch.equal(outs[i], want), (step, i)
+            if step == 2:
+                assert (want[21:] == 0).all() and not (want[:21] == 0).all()
+                s["table"][2, 0] = 3
+        assert not torch.equal(outs[0], outs[1])
